@@ -360,6 +360,100 @@ typedef struct {
 KREA_CUDA_API size_t krea_cuda_dit_block_workspace_bytes(const krea_cuda_dit_block_args* a);
 KREA_CUDA_API int krea_cuda_dit_block(krea_cuda* h, const krea_cuda_dit_block_args* a);
 
+/* ---- 4-bit floating point (no counterpart in the reference, whose smallest weights are int8, engine/src/metal.h:25-29) ----
+ * e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) with one scale for each block of values along K:
+ *   KREA_CUDA_FP4_MX  blocks of 32, scale 2^(floor(log2(amax)) - 2) stored as e8m0 (biased by 127, 2^-127 at least); larger
+ *                     values than 6 scales become 6 scales
+ *   KREA_CUDA_FP4_NV  blocks of 16, scale s = amax / (6 ts) rounded to e4m3 (448 at most), a value stands for e2m1 * s * ts;
+ *                     ts is one f32 for the whole tensor in device memory (NULL = 1), positive and finite.
+ *                     amax(tensor) / (6 * 448) uses the whole range.
+ * Every value is rounded once, to the nearest of the grid, a tie to the even code; a sign is kept.  A block that holds an
+ * infinity or a NaN gets the scale code NaN, and so becomes NaN as a whole, as do products with it.
+ * Packed rows: value k of a row in byte k / 2, the even one in the low bits; krea_cuda_fp4_row_bytes(K) = 16 * ceil(K / 32)
+ * bytes, values past K zero.  ldq, lda and ldw are in BYTES, multiples of 16.
+ * Scales: krea_cuda_fp4_scale_bytes bytes, tiles of 128 rows x 256 values, [row / 128][k / 256][4 blocks][row % 32]
+ * [row / 32 % 4][block % 4], zero past K and past the last row.  The product reads the scales past K: they must not be NaN. */
+#define KREA_CUDA_FP4_MX 0
+#define KREA_CUDA_FP4_NV 1
+KREA_CUDA_API size_t krea_cuda_fp4_row_bytes(int K);
+KREA_CUDA_API size_t krea_cuda_fp4_scale_bytes(int format, int rows, int K);
+/* bf16 -> 4 bits.  src is [rows, ld] with K values a row, or, when transposed, [K, ld] with output row r in its column r:
+ * the "input-major" weights of krea_cuda_gemm become the rows of W that krea_cuda_gemm_fp4 takes.  ld in elements. */
+typedef struct {
+  const void* src;
+  void* q;
+  void* scales;
+  const float* tensor_scale;
+  int rows, K;
+  int ld, ldq;
+  int format;
+  int transposed;
+} krea_cuda_fp4_quantize_args;
+KREA_CUDA_API int krea_cuda_fp4_quantize(krea_cuda* h, const krea_cuda_fp4_quantize_args* a);
+/* 4 bits -> bf16 [rows, ldo]: bf16(e2m1 * scale * ts).  Columns from K on are left as they were. */
+typedef struct {
+  const void* q;
+  const void* scales;
+  const float* tensor_scale;
+  void* out;
+  int rows, K;
+  int ldq, ldo;
+  int format;
+} krea_cuda_fp4_dequantize_args;
+KREA_CUDA_API int krea_cuda_fp4_dequantize(krea_cuda* h, const krea_cuda_fp4_dequantize_args* a);
+/* C[M, N] = A x W^T on packed rows A [M, lda] and W [N, ldw] of one format, fp32 accumulation, times both tensor scales.
+ * Epilogues and C as in krea_cuda_gemm: KREA_CUDA_EPI_BF16, _RESID_GATE, _SWIGLU, _F32, _GELU, _BIAS_BF16, _BIAS_F32
+ * (_QKNORM_ROPE is KREA_CUDA_E_UNSUPPORTED: krea_cuda_joint_attention normalises and rotates Q and K itself).  Any M and K;
+ * N and ldc multiples of 8, SwiGLU's N of 64.  The result depends on M, N and K only, not on what runs beside it. */
+typedef struct {
+  const void* A;
+  const void* a_scales;
+  const void* W;
+  const void* w_scales;
+  void* C;
+  int M, N, K;
+  int lda, ldw, ldc;
+  int format;
+  int epilogue;
+  const float* vec;
+  const float* a_tensor_scale;
+  const float* w_tensor_scale;
+} krea_cuda_gemm_fp4_args;
+KREA_CUDA_API int krea_cuda_gemm_fp4(krea_cuda* h, const krea_cuda_gemm_fp4_args* a);
+
+/* ---- the norms before and after a sublayer with its gate and residual scale, in one pass ----
+ *   r = post ? y * rsqrt(mean(y^2) + eps) * post : y;   x' = x_scale * x + gate * r;
+ *   h = x' * rsqrt(mean(x'^2) + eps) * mul + add
+ * which is DiT::layer's `x += gate1 * (ao Wo)` with the norm that follows it (engine/src/model.mm:379-381), and also covers
+ * blocks with a norm after the sublayer and a scaled residual.  x f32 [rows, ld_x]; y bf16 (f32 when y_f32) [rows, ld_y] or NULL
+ * (then x' = x_scale * x); x_out f32 [rows, ld_xo], may be x itself, NULL = not stored; h per `out`: bf16, f32, or packed 4-bit
+ * rows (ld_h in BYTES) with h_scales, quantised from the bf16 rounding of h; NULL = no second norm.  post f32 [width] (NULL =
+ * no norm of y).  gate, mul, add: f32 vectors of width, row r uses the one at (r / mod_rows) * mod_ld (mod_rows 0: the one at 0),
+ * so that every sample of a batch has its own; gate NULL = 1, add NULL = 0.  width a multiple of 8, 32768 at most. */
+#define KREA_CUDA_OUT_BF16 0
+#define KREA_CUDA_OUT_F32 1
+#define KREA_CUDA_OUT_FP4_MX 2
+#define KREA_CUDA_OUT_FP4_NV 3
+typedef struct {
+  const float* x;
+  const void* y;
+  float* x_out;
+  void* h;
+  void* h_scales;
+  const float* h_tensor_scale;
+  const float* post;
+  const float* gate;
+  const float* mul;
+  const float* add;
+  int rows, width;
+  int ld_x, ld_y, ld_xo, ld_h;
+  int mod_rows, mod_ld;
+  float x_scale, eps;
+  int y_f32;
+  int out;
+} krea_cuda_gated_norm_args;
+KREA_CUDA_API int krea_cuda_gated_norm(krea_cuda* h, const krea_cuda_gated_norm_args* a);
+
 /* ---- `.qw` weight files (the reference's WeightFile, engine/src/weights.h:26-75, weights.mm:16-81; format
  * written by tools/convert.py:49-89) ----
  * The on-disk format that supplies the path's QK-norm weights `L<l>.qn` / `L<l>.kn` (f32[128]):

@@ -13,6 +13,8 @@ PART_FIRST, PART_MID, PART_LAST = 0, 1, 2
 OK, E_ARG, E_UNSUPPORTED, E_CUDA, E_DEVICE, E_NOMEM, E_COMM, E_TIMEOUT = 0, -1, -2, -3, -4, -5, -6, -7
 ROPE_PAIRS, ROPE_HALF, ROPE_NONE = 0, 1, 2
 EPI_BF16, EPI_QKNORM_ROPE, EPI_RESID_GATE, EPI_SWIGLU, EPI_F32, EPI_GELU, EPI_BIAS_BF16, EPI_BIAS_F32 = 0, 1, 2, 3, 4, 5, 6, 7
+FP4_MX, FP4_NV = 0, 1
+OUT_BF16, OUT_F32, OUT_FP4_MX, OUT_FP4_NV = 0, 1, 2, 3
 STATIC_SCRATCH_BYTES = 32 << 20   # KREA_CUDA_STATIC_SCRATCH_BYTES
 DIST_ID_BYTES = 128                # KREA_CUDA_DIST_ID_BYTES
 
@@ -83,6 +85,29 @@ class DitBlockArgs(ctypes.Structure):
                 ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("use_big_dim", _int), ("big_dim", _int)]
 
 
+class Fp4QuantizeArgs(ctypes.Structure):
+    _fields_ = [("src", _vp), ("q", _vp), ("scales", _vp), ("tensor_scale", _vp), ("rows", _int), ("K", _int),
+                ("ld", _int), ("ldq", _int), ("format", _int), ("transposed", _int)]
+
+
+class Fp4DequantizeArgs(ctypes.Structure):
+    _fields_ = [("q", _vp), ("scales", _vp), ("tensor_scale", _vp), ("out", _vp), ("rows", _int), ("K", _int),
+                ("ldq", _int), ("ldo", _int), ("format", _int)]
+
+
+class GemmFp4Args(ctypes.Structure):
+    _fields_ = [("A", _vp), ("a_scales", _vp), ("W", _vp), ("w_scales", _vp), ("C", _vp), ("M", _int), ("N", _int), ("K", _int),
+                ("lda", _int), ("ldw", _int), ("ldc", _int), ("format", _int), ("epilogue", _int), ("vec", _vp),
+                ("a_tensor_scale", _vp), ("w_tensor_scale", _vp)]
+
+
+class GatedNormArgs(ctypes.Structure):
+    _fields_ = [("x", _vp), ("y", _vp), ("x_out", _vp), ("h", _vp), ("h_scales", _vp), ("h_tensor_scale", _vp),
+                ("post", _vp), ("gate", _vp), ("mul", _vp), ("add", _vp), ("rows", _int), ("width", _int),
+                ("ld_x", _int), ("ld_y", _int), ("ld_xo", _int), ("ld_h", _int), ("mod_rows", _int), ("mod_ld", _int),
+                ("x_scale", ctypes.c_float), ("eps", ctypes.c_float), ("y_f32", _int), ("out", _int)]
+
+
 class QwInfo(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("dtype", ctypes.c_char_p), ("rank", _int), ("shape", _i64 * 8),
                 ("offset", ctypes.c_uint64), ("nbytes", ctypes.c_uint64)]
@@ -128,6 +153,12 @@ SYMBOLS = {
     "krea_cuda_dit_block_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(DitBlockArgs)]),
     "krea_cuda_dit_block": (_int, [_vp, ctypes.POINTER(DitBlockArgs)]),
     "krea_cuda_layerwise_attn": (_int, [_vp, ctypes.POINTER(LayerwiseArgs)]),
+    "krea_cuda_fp4_row_bytes": (ctypes.c_size_t, [_int]),
+    "krea_cuda_fp4_scale_bytes": (ctypes.c_size_t, [_int, _int, _int]),
+    "krea_cuda_fp4_quantize": (_int, [_vp, ctypes.POINTER(Fp4QuantizeArgs)]),
+    "krea_cuda_fp4_dequantize": (_int, [_vp, ctypes.POINTER(Fp4DequantizeArgs)]),
+    "krea_cuda_gemm_fp4": (_int, [_vp, ctypes.POINTER(GemmFp4Args)]),
+    "krea_cuda_gated_norm": (_int, [_vp, ctypes.POINTER(GatedNormArgs)]),
     "krea_cuda_qw_open": (_vp, [ctypes.c_char_p, ctypes.c_char_p, _int]),
     "krea_cuda_qw_close": (None, [_vp]),
     "krea_cuda_qw_count": (_int, [_vp]),

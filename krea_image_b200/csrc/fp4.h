@@ -1,0 +1,85 @@
+// Kernel-facing side of the 4-bit operators and of the gated norm: parameters and launchers, shared by their kernels
+// and by the host code of the C ABI.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace krea {
+
+// rows [rows, K] of bf16 -> packed e2m1 rows + block scales.  src: row-major [rows, ld], or [K, ld] when transposed.
+struct Fp4QuantParams {
+  const __nv_bfloat16* src;
+  uint8_t* q;
+  uint8_t* scales;
+  const float* tensor_scale;    // nullptr = 1 (and always for the MX format)
+  int rows, K;
+  int64_t ld, ldq;
+  int mx;                       // 1: blocks of 32, e8m0 scales; 0: blocks of 16, e4m3 scales
+};
+cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, bool transposed, cudaStream_t stream);
+
+struct Fp4DequantParams {
+  const uint8_t* q;
+  const uint8_t* scales;
+  const float* tensor_scale;
+  __nv_bfloat16* out;
+  int rows, K;
+  int64_t ldq, ldo;
+  int mx;
+};
+cudaError_t launch_fp4_dequantize(const Fp4DequantParams& p, cudaStream_t stream);
+
+struct Fp4GemmParams {
+  void* C;
+  int64_t ldc;
+  int M, N, K;
+  int epi;                      // the KREA_CUDA_EPI_* value
+  int mx;
+  const float* vec;
+  const float* a_ts;            // device scalars, nullptr = 1
+  const float* w_ts;
+  uint32_t* status;
+  int group_m;                  // set by the launcher: row blocks per group of the tile order
+};
+// Tensor maps of one operand: values [rows, packed row] in bytes, 128-byte swizzled boxes of 128 bytes x `box_rows`
+// rows; scales [row tile][256-value chunk][chunk bytes] as 8-byte words.
+struct Fp4Operand {
+  const void* values;
+  const void* scales;
+  int rows;
+  int64_t ld;
+};
+struct Fp4GemmPlan {
+  bool pair;                    // 256 x 256 tiles on CTA pairs; else 128 weight columns x tn rows a CTA
+  int tn;                       // rows of A a CTA takes (columns of its tensor-core tile)
+  int split;                    // CTAs of a cluster that share one tile's K
+};
+Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms);
+typedef CUresult (*Fp4EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+cudaError_t launch_gemm_fp4(const Fp4GemmPlan& plan, const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p,
+                            int sms, cudaStream_t stream);
+
+struct GatedNormParams {
+  const float* x;
+  const void* y;                // bf16, or f32 when y_f32; nullptr = x' is x_scale * x
+  float* x_out;                 // nullptr = not stored
+  void* h;                      // nullptr = no second norm
+  uint8_t* h_scales;
+  const float* h_ts;
+  const float* post;
+  const float* gate;
+  const float* mul;
+  const float* add;
+  int rows, width;
+  int64_t ld_x, ld_y, ld_xo, ld_h;   // elements; ld_h in bytes for the 4-bit forms
+  int mod_rows;                 // rows that share one vector of gate, mul and add (0 = all)
+  int64_t mod_ld;
+  float x_scale, eps;
+  int y_f32, out;               // out: the KREA_CUDA_OUT_* value
+};
+cudaError_t launch_gated_norm(const GatedNormParams& p, cudaStream_t stream);
+
+}  // namespace krea

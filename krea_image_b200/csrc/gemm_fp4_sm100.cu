@@ -1,0 +1,336 @@
+// 4-bit GEMM for B200 (sm_100a): C[M, N] = (A . sA) x (W . sW)^T on packed e2m1 rows with block scales, both operands
+// with K innermost, fp32 accumulation, the epilogues of the bf16 GEMM.
+//
+// tcgen05.mma kind::mxf4nvf4 (NV, a scale each 16 values) and kind::mxf4 (MX, each 32) multiply 64 values of K an
+// instruction and take the scales from tensor memory: 32 lanes x 4 columns of words for 128 rows, repeated in the four
+// lane quarters.  The scale storage (fp4_block.cuh) is that order, so a 512-byte piece goes from memory to shared memory by
+// TMA and to tensor memory by one tcgen05.cp, untouched.
+//
+// Two kernels:
+//   gemm_fp4_rows_sm100   few rows of A: the 128 tensor-core rows are columns of C (rows of W), the rows of A (16 to 128)
+//                         are its columns, so the weights stream through once and no tensor-core row idles; the CTAs of a
+//                         cluster share K and add their parts through shared memory, in a fixed order.
+//   gemm_fp4_pair_sm100   many rows: 256 x 256 tiles on CTA pairs (cta_group::2), persistent, like the bf16 kernel.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <mutex>
+
+#include "../../include/krea_cuda.h"
+#include "fp4.h"
+#include "sm100_pair.cuh"
+#include "sm100_ptx.cuh"
+
+namespace krea {
+
+namespace fp4g {
+enum : uint32_t { SITE_FULL = 21, SITE_EMPTY = 22, SITE_ACC_FULL = 23, SITE_ACC_EMPTY = 24 };
+constexpr int KB = 256;                              // values of K a stage: one 128-byte row of packed values
+constexpr int ROW_TILE_BYTES = 128 * 128;            // 128 rows of a stage
+__host__ __device__ constexpr int scale_chunk(bool mx) { return mx ? 1024 : 2048; }   // scale bytes of 128 rows x 256 values
+__host__ __device__ constexpr int scale_pieces(bool mx) { return mx ? 2 : 4; }        // 512-byte pieces (4 columns of tensor memory) among them
+
+// instruction descriptor of the block-scaled kinds: e2m1 x e2m1, fp32 accumulator, both operands K-major
+__host__ __device__ constexpr uint32_t idesc(bool mx, int M, int N) {
+  return (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((mx ? 1u : 0u) << 23) | ((uint32_t)(M >> 4) << 24);
+}
+// which bytes of the scale words an MX instruction takes: 0 the lower two, 2 the upper two (bits 29-30: A, 4-5: B)
+__host__ __device__ constexpr uint32_t idesc_sf(uint32_t id) { return (id << 29) | (id << 4); }
+
+template <bool MX, int CTAS>
+__device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc_, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  if constexpr (MX && CTAS == 1)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc_), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+  else if constexpr (MX)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc_), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+  else if constexpr (CTAS == 1)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc_), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc_), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// 512 bytes of scales, shared -> tensor memory: 32 lanes x 16 bytes, repeated in the four lane quarters
+template <int CTAS>
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t saddr16) {
+  // no swizzle, groups of 8 rows x 16 bytes 128 bytes apart
+  const uint64_t desc = make_desc(saddr16, (128u >> 4) | (1u << 14));
+  if constexpr (CTAS == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ float tensor_scale(const Fp4GemmParams& p) {
+  float s = 1.f;
+  if (p.a_ts) s *= __ldg(p.a_ts);
+  if (p.w_ts) s *= __ldg(p.w_ts);
+  return s;
+}
+__device__ __forceinline__ float gelu_tanh(float x) { return 0.5f * x * (1.0f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x))); }
+
+// ---------------------------------------------------------------------------------------------- few rows
+template <bool MX, int TN>
+struct RowsCfg {
+  static constexpr int X_BYTES = ROW_TILE_BYTES, Y_BYTES = TN * 128, S_BYTES = scale_chunk(MX);
+  static constexpr int STAGE_BYTES = X_BYTES + Y_BYTES + 2 * S_BYTES;
+  // two CTAs an SM, in shared memory (228 KB, 1 KB of it taken by each CTA) as in tensor memory (512 columns)
+  static constexpr int FIT = (228 * 1024 / 2 - 1024 - 256 - 1024) / STAGE_BYTES, STAGES = FIT < 5 ? FIT : 5;
+  static constexpr int SF_COLS = 2 * 4 * scale_pieces(MX);     // tensor-memory columns of a stage's scales
+  static constexpr int ACC_COLS = TN < 32 ? 32 : TN;
+  static constexpr int TMEM_USED = ACC_COLS + STAGES * SF_COLS;
+  static constexpr int TMEM_COLS = TMEM_USED <= 128 ? 128 : TMEM_USED <= 256 ? 256 : 512;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 256 + 1024;
+};
+constexpr int ROWS_THREADS = 192;   // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+}  // namespace fp4g
+
+template <bool MX, int TN>
+__global__ void __launch_bounds__(fp4g::ROWS_THREADS)
+gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs, const __grid_constant__ CUtensorMap tmW,
+                    const __grid_constant__ CUtensorMap tmWs, const Fp4GemmParams p) {
+  using namespace fp4g;
+  using C = RowsCfg<MX, TN>;
+  constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES, PIECES = scale_pieces(MX);
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = (uint64_t*)(smem + STAGES * STAGE_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
+  volatile uint32_t* abort_word = (volatile uint32_t*)(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t split = gridDim.z, rank = blockIdx.z;       // the cluster is the grid's z axis
+  const int n0 = blockIdx.x * 128, m0 = blockIdx.y * TN;
+  const int kblocks = (p.K + KB - 1) / KB;
+  const int kb0 = (int)((int64_t)kblocks * rank / split), kb1 = (int)((int64_t)kblocks * (rank + 1) / split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    abort_word[0] = (p.status != nullptr && *p.status != 0u) ? 0xFFu : 0u;
+    abort_word[1] = 0u;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot, sf_base = tmem_base + C::ACC_COLS;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tmW);
+      tma_prefetch_desc(&tmWs);
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmAs);
+      uint32_t n = 0;
+      for (int kb = kb0; kb < kb1 && *abort_word == 0u; kb++, n++) {
+        const int s = n % STAGES;
+        if (!mbar_wait(&empty[s], ((n / STAGES) & 1) ^ 1, abort_word, SITE_EMPTY)) break;
+        uint8_t* st = smem + s * STAGE_BYTES;
+        mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
+        tma_load_3d(st, &tmW, &full[s], kb * 128, n0, 0);
+        tma_load_3d(st + C::X_BYTES, &tmA, &full[s], kb * 128, m0, 0);
+        tma_load_3d(st + C::X_BYTES + C::Y_BYTES, &tmWs, &full[s], 0, kb, n0 >> 7);
+        tma_load_3d(st + C::X_BYTES + C::Y_BYTES + C::S_BYTES, &tmAs, &full[s], 0, kb, m0 >> 7);
+      }
+      // nothing may still be in flight into this CTA's shared memory when it exits
+      if (*abort_word != 0u) {
+        for (uint32_t i = (n > STAGES ? n - STAGES : 0); i < n; i++) mbar_wait_slow(&full[i % STAGES], (i / STAGES) & 1, abort_word + 1, SITE_FULL);
+      }
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    constexpr uint32_t HI = desc_hi(1024), ID = idesc(MX, 128, TN);
+    const uint32_t smem16 = smem_u32(smem) >> 4;
+    uint32_t n = 0;
+    for (int kb = kb0; kb < kb1; kb++, n++) {
+      const int s = n % STAGES;
+      if (!mbar_wait(&full[s], (n / STAGES) & 1, abort_word, SITE_FULL)) break;
+      tc_fence_after();
+      const uint32_t x = smem16 + s * (STAGE_BYTES >> 4), y = x + (C::X_BYTES >> 4), sx = y + (C::Y_BYTES >> 4), sy = sx + (C::S_BYTES >> 4);
+      const uint32_t tx = sf_base + s * C::SF_COLS, ty = tx + 4 * PIECES;
+      if (leader) {
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) {
+          copy_scales<1>(tx + 4 * j, sx + j * 32);
+          copy_scales<1>(ty + 4 * j, sy + j * 32);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int piece = MX ? j >> 1 : j;
+          mma<MX, 1>(tmem_base, make_desc(x + j * 2, HI), make_desc(y + j * 2, HI), ID | idesc_sf(MX ? (j & 1) * 2 : 0), tx + 4 * piece, ty + 4 * piece, (kb > kb0 || j > 0) ? 1u : 0u);
+        }
+        umma_commit(&empty[s]);
+      }
+      __syncwarp();
+    }
+    if (leader) umma_commit(acc_full);
+    __syncwarp();
+  }
+  // tensor memory -> shared memory as [row of A][128 columns of C] f32, over the stages, which nothing uses any more
+  float* part = (float*)smem;
+  if (warp >= 2) {
+    const int quarter = warp & 3;
+    const bool ok = mbar_wait(acc_full, 0, abort_word, SITE_ACC_FULL);
+    tc_fence_after();
+    if (ok) {
+#pragma unroll 1
+      for (int c0 = 0; c0 < TN; c0 += 32) {
+        if (m0 + c0 >= p.M) break;
+        uint32_t v[32];
+        tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + c0, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+          if (TN >= 32 || e < TN) part[(c0 + e) * 128 + quarter * 32 + lane] = __uint_as_float(v[e]);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncwarp();
+  __syncthreads();
+  if (split > 1) cluster_sync_all();
+
+  // every CTA of the cluster finishes its share of the tile: 8 columns of one row at a time, parts added in rank order
+  const bool swiglu = p.epi == KREA_CUDA_EPI_SWIGLU;
+  const int rows = min(TN, p.M - m0), units_row = swiglu ? 8 : 16;
+  const float alpha = tensor_scale(p);
+  const bool live = *abort_word == 0u;
+  for (int u = rank * ROWS_THREADS + threadIdx.x; live && u < rows * units_row; u += split * ROWS_THREADS) {
+    const int r = u / units_row, uc = u % units_row;
+    const int c = swiglu ? (uc >> 2) * 64 + (uc & 3) * 8 : uc * 8;       // first of the tile's columns (SwiGLU: of the gate's)
+    if (n0 + c >= p.N) continue;
+    float f[8], g[8];
+    auto sum = [&](int col, float* o) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e] = 0.f;
+      for (uint32_t q = 0; q < split; q++) {
+        float4 a, b;
+        if (split > 1) {
+          const uint32_t at = mapa(smem_u32(part + r * 128 + col), q);
+          a = ld_cluster_f32x4(at);
+          b = ld_cluster_f32x4(at + 16);
+        } else {
+          a = *(const float4*)(part + r * 128 + col);
+          b = *(const float4*)(part + r * 128 + col + 4);
+        }
+        o[0] += a.x; o[1] += a.y; o[2] += a.z; o[3] += a.w; o[4] += b.x; o[5] += b.y; o[6] += b.z; o[7] += b.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e] *= alpha;
+    };
+    sum(c, f);
+    int64_t col = n0 + c;
+    if (swiglu) {
+      sum(c + 32, g);
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[e] = f[e] * sigmoid_approx(f[e]) * g[e];
+      col = ((n0 + c) >> 6) * 32 + (uc & 3) * 8;
+    }
+    if (p.epi == KREA_CUDA_EPI_BIAS_BF16 || p.epi == KREA_CUDA_EPI_BIAS_F32) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[e] += __ldg(p.vec + col + e);
+    } else if (p.epi == KREA_CUDA_EPI_GELU) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[e] = gelu_tanh(f[e]);
+    }
+    const int64_t at = (int64_t)(m0 + r) * p.ldc + col;
+    if (p.epi == KREA_CUDA_EPI_RESID_GATE) {
+      float4* o = (float4*)((float*)p.C + at);
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const float4 gt = p.vec ? __ldg((const float4*)(p.vec + col) + e) : make_float4(1.f, 1.f, 1.f, 1.f);
+        float4 x = o[e];
+        x.x = fmaf(gt.x, f[4 * e], x.x); x.y = fmaf(gt.y, f[4 * e + 1], x.y); x.z = fmaf(gt.z, f[4 * e + 2], x.z); x.w = fmaf(gt.w, f[4 * e + 3], x.w);
+        o[e] = x;
+      }
+    } else if (p.epi == KREA_CUDA_EPI_F32 || p.epi == KREA_CUDA_EPI_BIAS_F32) {
+      float4* o = (float4*)((float*)p.C + at);
+      o[0] = make_float4(f[0], f[1], f[2], f[3]);
+      o[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+      *(uint4*)((__nv_bfloat16*)p.C + at) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (split > 1) cluster_sync_all();       // nobody leaves while the others still read its part
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+  if (threadIdx.x == 0 && p.status != nullptr) {
+    const uint32_t a = *abort_word;
+    if (a != 0u && a != 0xFFu) atomicCAS(p.status, 0u, a | ((blockIdx.x & 0xFFFu) << 8));
+  }
+}
+
+template <bool MX, int TN>
+static cudaError_t launch_rows_variant(const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p, int split,
+                                       cudaStream_t stream) {
+  using namespace fp4g;
+  static bool configured[64] = {};
+  static std::mutex configure_mutex;       // handles on several threads may launch at the same time
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> lock(configure_mutex);
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+      cudaError_t e = cudaFuncSetAttribute(gemm_fp4_rows_sm100<MX, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsCfg<MX, TN>::SMEM);
+      if (e != cudaSuccess) return e;
+      if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.N + 127) / 128), (unsigned)((p.M + TN - 1) / TN), (unsigned)split);
+  cfg.blockDim = dim3(ROWS_THREADS);
+  cfg.dynamicSmemBytes = RowsCfg<MX, TN>::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = (unsigned)split;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, gemm_fp4_rows_sm100<MX, TN>, tmA, tmAs, tmW, tmWs, p);
+}
+
+Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms) {
+  (void)mx;
+  Fp4GemmPlan plan{};
+  plan.tn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + plan.tn - 1) / plan.tn);
+  const int kblocks = (K + fp4g::KB - 1) / fp4g::KB;
+  // enough CTAs to fill the SMs, at least two stages of K each
+  plan.split = 1;
+  while (plan.split < 8 && tiles * plan.split * 2 <= 2 * sms && kblocks >= plan.split * 4) plan.split *= 2;
+  return plan;
+}
+
+cudaError_t launch_gemm_fp4(const Fp4GemmPlan& plan, const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p,
+                            int sms, cudaStream_t stream) {
+  (void)sms;
+  if (p.M <= 0 || p.N <= 0 || p.K <= 0) return cudaSuccess;
+#define KREA_ROWS(TN) return p.mx ? launch_rows_variant<true, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, stream) : launch_rows_variant<false, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, stream)
+  switch (plan.tn) {
+    case 16: KREA_ROWS(16);
+    case 32: KREA_ROWS(32);
+    case 64: KREA_ROWS(64);
+    default: KREA_ROWS(128);
+  }
+#undef KREA_ROWS
+}
+
+}  // namespace krea

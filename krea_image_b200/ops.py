@@ -181,6 +181,34 @@ class KreaCuda:
         a = B.DequantArgs(_ptr(wq), _ptr(scales), _ptr(out), K, N, N if ldq is None else ldq, N if lds is None else lds, N if ldo is None else ldo)
         self._check(self.lib.krea_cuda_dequant_q8(self.h, ctypes.byref(a)))
 
+    # ---- 4-bit rows: e2m1 values with block scales (format B.FP4_MX or B.FP4_NV) ---------------------
+    def fp4_quantize(self, src, q, scales, rows, K, ld, ldq, format=B.FP4_MX, *, tensor_scale=None, transposed=False):
+        """bf16 [rows, ld] (transposed: [K, ld], output row r in column r) -> packed rows q [rows, ldq bytes] and
+        fp4_scale_bytes(format, rows, K) bytes of scales; tensor_scale: device f32[1], FP4_NV only."""
+        a = B.Fp4QuantizeArgs(_ptr(src), _ptr(q), _ptr(scales), _ptr(tensor_scale), rows, K, ld, ldq, format, int(bool(transposed)))
+        self._check(self.lib.krea_cuda_fp4_quantize(self.h, ctypes.byref(a)))
+
+    def fp4_dequantize(self, q, scales, out, rows, K, ldq, ldo, format=B.FP4_MX, *, tensor_scale=None):
+        """Packed rows -> bf16 [rows, ldo]."""
+        a = B.Fp4DequantizeArgs(_ptr(q), _ptr(scales), _ptr(tensor_scale), _ptr(out), rows, K, ldq, ldo, format)
+        self._check(self.lib.krea_cuda_fp4_dequantize(self.h, ctypes.byref(a)))
+
+    def gemm_fp4(self, A, a_scales, W, w_scales, C, M, N, K, lda, ldw, ldc, format=B.FP4_MX, *, epilogue=B.EPI_BF16, vec=None,
+                 a_tensor_scale=None, w_tensor_scale=None):
+        """C[M, N] = A[M, K] x W[N, K]^T on packed rows (lda, ldw in bytes), with the epilogues of gemm()."""
+        a = B.GemmFp4Args(_ptr(A), _ptr(a_scales), _ptr(W), _ptr(w_scales), _ptr(C), M, N, K, lda, ldw, ldc, format, epilogue,
+                          _ptr(vec), _ptr(a_tensor_scale), _ptr(w_tensor_scale))
+        self._check(self.lib.krea_cuda_gemm_fp4(self.h, ctypes.byref(a)))
+
+    def gated_norm(self, x, y, x_out, h, rows, width, ld_x, ld_y, ld_xo, ld_h, *, post=None, gate=None, mul=None, add=None,
+                   x_scale=1.0, eps=1e-6, mod_rows=0, mod_ld=0, y_f32=False, out=B.OUT_BF16, h_scales=None, h_tensor_scale=None):
+        """x_out = x_scale * x + gate * (post-norm of y); h = norm(x_out) * mul + add, stored as `out` says (B.OUT_*;
+        ld_h in bytes for the 4-bit ones)."""
+        a = B.GatedNormArgs(_ptr(x), _ptr(y), _ptr(x_out), _ptr(h), _ptr(h_scales), _ptr(h_tensor_scale), _ptr(post), _ptr(gate),
+                            _ptr(mul), _ptr(add), rows, width, ld_x, ld_y, ld_xo, ld_h, mod_rows, mod_ld, x_scale, eps,
+                            int(bool(y_f32)), out)
+        self._check(self.lib.krea_cuda_gated_norm(self.h, ctypes.byref(a)))
+
     def rms_norm(self, x, mul, add, y, rows, width, ld_in, ld_out, eps, f32_out=False):
         """Metal::rms_norm (engine/src/metal.h:75-77): same argument order."""
         a = B.RmsNormArgs(_ptr(x), _ptr(mul), _ptr(add), _ptr(y), rows, width, ld_in, ld_out, eps, int(bool(f32_out)))
@@ -259,6 +287,16 @@ class KreaCuda:
         a = B.SeqParArgs(_ptr(Q), _ptr(K), _ptr(V), _ptr(O), seq, heads, group, ldq, ldk, ldv, ldo,
                          _ptr(wq), _ptr(wk), _ptr(cos), _ptr(sin), eps, rope_mode)
         self._check(self.lib.krea_cuda_seqpar_joint_attention(self.h, ctypes.byref(a)))
+
+
+def fp4_row_bytes(K) -> int:
+    """Bytes of one packed row of K 4-bit values."""
+    return int(B.load().krea_cuda_fp4_row_bytes(K))
+
+
+def fp4_scale_bytes(format, rows, K) -> int:
+    """Bytes of the block scales of [rows, K]; 0 for a bad format or an empty matrix."""
+    return int(B.load().krea_cuda_fp4_scale_bytes(format, rows, K))
 
 
 def rope_tables_ref3axis(T, gh, gw):
