@@ -43,22 +43,15 @@ struct Fp4GemmParams {
   uint32_t* status;
   int group_m;                  // set by the launcher: row blocks per group of the tile order
 };
-// Tensor maps of one operand: values [rows, packed row] in bytes, 128-byte swizzled boxes of 128 bytes x `box_rows`
-// rows; scales [row tile][256-value chunk][chunk bytes] as 8-byte words.
-struct Fp4Operand {
-  const void* values;
-  const void* scales;
-  int rows;
-  int64_t ld;
-};
 struct Fp4GemmPlan {
   bool pair;                    // 256 x 256 tiles on CTA pairs; else 128 weight columns x tn rows a CTA
   int tn;                       // rows of A a CTA takes (columns of its tensor-core tile)
   int split;                    // CTAs of a cluster that share one tile's K
 };
-Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms);
-typedef CUresult (*Fp4EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// force: 0 = choose by size, 1 = few-rows kernel, 2 = CTA pairs
+Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force);
+// Tensor maps: values [rows, packed row] in bytes, 128-byte swizzled boxes of 128 bytes x 128 rows (A of the few-rows kernel:
+// plan.tn rows); scales [row tile][256-value chunk][chunk] as 8-byte words, a box one chunk of one row tile (W of the pair kernel: of two)
 cudaError_t launch_gemm_fp4(const Fp4GemmPlan& plan, const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p,
                             int sms, cudaStream_t stream);
 

@@ -77,7 +77,7 @@ int krea_cuda_gemm_fp4(krea_cuda* h, const krea_cuda_gemm_fp4_args* a) {
     h->sm_count = prop.multiProcessorCount;
   }
   const bool mx = a->format == KREA_CUDA_FP4_MX;
-  const Fp4GemmPlan plan = plan_gemm_fp4(a->M, a->N, a->K, mx, h->sm_count);
+  const Fp4GemmPlan plan = plan_gemm_fp4(a->M, a->N, a->K, mx, h->sm_count, h->fp4_tile);
   CUtensorMap tmA, tmAs, tmW, tmWs;
   int rc;
   if ((rc = make_values_map(h, &tmA, a->A, a->M, a->K, a->lda, plan.pair ? 128 : plan.tn, "A"))) return rc;

@@ -71,6 +71,81 @@ __device__ __forceinline__ float tensor_scale(const Fp4GemmParams& p) {
 }
 __device__ __forceinline__ float gelu_tanh(float x) { return 0.5f * x * (1.0f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x))); }
 
+// Everything after the sum for 8 columns of one row (SwiGLU apart), and their store
+__device__ __forceinline__ void finish8(const Fp4GemmParams& p, float* f, int row, int col) {
+  if (p.epi == KREA_CUDA_EPI_BIAS_BF16 || p.epi == KREA_CUDA_EPI_BIAS_F32) {
+    const float4 a = __ldg((const float4*)(p.vec + col)), b = __ldg((const float4*)(p.vec + col) + 1);
+    f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+  } else if (p.epi == KREA_CUDA_EPI_GELU) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = gelu_tanh(f[e]);
+  }
+  const int64_t at = (int64_t)row * p.ldc + col;
+  if (p.epi == KREA_CUDA_EPI_RESID_GATE) {
+    float4* o = (float4*)((float*)p.C + at);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const float4 gt = p.vec ? __ldg((const float4*)(p.vec + col) + e) : make_float4(1.f, 1.f, 1.f, 1.f);
+      float4 x = o[e];
+      x.x = fmaf(gt.x, f[4 * e], x.x); x.y = fmaf(gt.y, f[4 * e + 1], x.y); x.z = fmaf(gt.z, f[4 * e + 2], x.z); x.w = fmaf(gt.w, f[4 * e + 3], x.w);
+      o[e] = x;
+    }
+  } else if (p.epi == KREA_CUDA_EPI_F32 || p.epi == KREA_CUDA_EPI_BIAS_F32) {
+    float4* o = (float4*)((float*)p.C + at);
+    o[0] = make_float4(f[0], f[1], f[2], f[3]);
+    o[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    *(uint4*)((__nv_bfloat16*)p.C + at) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  }
+}
+
+// Epilogue of a thread of the pair kernel: columns [col0, col0 + 128) of one row of C, as far as N goes (N a multiple of 8,
+// of 64 with SwiGLU).
+__device__ __forceinline__ void pair_store(const Fp4GemmParams& p, const uint32_t* v, int row, int col0, float alpha) {
+  const int left = p.N - col0;
+  if (p.epi == KREA_CUDA_EPI_SWIGLU) {
+    __nv_bfloat16* o = (__nv_bfloat16*)p.C + (int64_t)row * p.ldc + (col0 >> 1);
+#pragma unroll
+    for (int c = 0; c < 128; c += 64) {
+      if (c >= left) break;
+      uint32_t pk[16];
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        const float g0 = __uint_as_float(v[c + 2 * e]) * alpha, g1 = __uint_as_float(v[c + 2 * e + 1]) * alpha;
+        const float u0 = __uint_as_float(v[c + 32 + 2 * e]) * alpha, u1 = __uint_as_float(v[c + 33 + 2 * e]) * alpha;
+        pk[e] = pack_bf16x2(g0 * sigmoid_approx(g0) * u0, g1 * sigmoid_approx(g1) * u1);
+      }
+      if ((((uintptr_t)(o + (c >> 1))) & 31u) == 0) {
+        st_global_32B(o + (c >> 1), pk);
+        st_global_32B(o + (c >> 1) + 16, pk + 8);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; q++) *(uint4*)(o + (c >> 1) + q * 8) = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+      }
+    }
+    return;
+  }
+  if (p.epi == KREA_CUDA_EPI_BF16 && left >= 128 && (((uintptr_t)p.C | (uintptr_t)(p.ldc * 2)) & 31u) == 0) {
+    __nv_bfloat16* o = (__nv_bfloat16*)p.C + (int64_t)row * p.ldc + col0;
+#pragma unroll
+    for (int c = 0; c < 128; c += 16) {
+      uint32_t pk[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) pk[e] = pack_bf16x2(__uint_as_float(v[c + 2 * e]) * alpha, __uint_as_float(v[c + 2 * e + 1]) * alpha);
+      st_global_32B(o + c, pk);
+    }
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < 128; c += 8) {
+    if (c >= left) break;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = __uint_as_float(v[c + e]) * alpha;
+    finish8(p, f, row, col0 + c);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------- few rows
 template <bool MX, int TN>
 struct RowsCfg {
@@ -231,37 +306,14 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       for (int e = 0; e < 8; e++) o[e] *= alpha;
     };
     sum(c, f);
-    int64_t col = n0 + c;
+    int col = n0 + c;
     if (swiglu) {
       sum(c + 32, g);
 #pragma unroll
       for (int e = 0; e < 8; e++) f[e] = f[e] * sigmoid_approx(f[e]) * g[e];
       col = ((n0 + c) >> 6) * 32 + (uc & 3) * 8;
     }
-    if (p.epi == KREA_CUDA_EPI_BIAS_BF16 || p.epi == KREA_CUDA_EPI_BIAS_F32) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) f[e] += __ldg(p.vec + col + e);
-    } else if (p.epi == KREA_CUDA_EPI_GELU) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) f[e] = gelu_tanh(f[e]);
-    }
-    const int64_t at = (int64_t)(m0 + r) * p.ldc + col;
-    if (p.epi == KREA_CUDA_EPI_RESID_GATE) {
-      float4* o = (float4*)((float*)p.C + at);
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const float4 gt = p.vec ? __ldg((const float4*)(p.vec + col) + e) : make_float4(1.f, 1.f, 1.f, 1.f);
-        float4 x = o[e];
-        x.x = fmaf(gt.x, f[4 * e], x.x); x.y = fmaf(gt.y, f[4 * e + 1], x.y); x.z = fmaf(gt.z, f[4 * e + 2], x.z); x.w = fmaf(gt.w, f[4 * e + 3], x.w);
-        o[e] = x;
-      }
-    } else if (p.epi == KREA_CUDA_EPI_F32 || p.epi == KREA_CUDA_EPI_BIAS_F32) {
-      float4* o = (float4*)((float*)p.C + at);
-      o[0] = make_float4(f[0], f[1], f[2], f[3]);
-      o[1] = make_float4(f[4], f[5], f[6], f[7]);
-    } else {
-      *(uint4*)((__nv_bfloat16*)p.C + at) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-    }
+    finish8(p, f, m0 + r, col);
   }
   __syncwarp();
   __syncthreads();
@@ -276,22 +328,206 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
 }
 
+// ---------------------------------------------------------------------------------------------- many rows
+namespace fp4g {
+template <bool MX>
+struct PairCfg {
+  static constexpr int S_BYTES = scale_chunk(MX);
+  // this CTA's 128 rows of A and of W (half of the tile's columns), the scales of its rows of A and of all 256 columns
+  static constexpr int STAGE_BYTES = 2 * ROW_TILE_BYTES + 3 * S_BYTES;
+  static constexpr int STAGES = MX ? 6 : 5;
+  static constexpr int SF_COLS = 3 * 4 * scale_pieces(MX);
+  static constexpr int ACC_COLS = 256;
+  static constexpr int TMEM_COLS = 512;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 256 + 1024;
+  static_assert(ACC_COLS + STAGES * SF_COLS <= TMEM_COLS && SMEM <= 227 * 1024, "tile does not fit");
+};
+constexpr int PAIR_THREADS = 384;   // warp 0 TMA, warp 1 MMA, warps 4-11 epilogue (two for each quarter of the tensor-memory lanes)
+}  // namespace fp4g
+
+template <bool MX>
+__global__ void __launch_bounds__(fp4g::PAIR_THREADS, 1)
+gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs, const __grid_constant__ CUtensorMap tmW,
+                    const __grid_constant__ CUtensorMap tmWs, const Fp4GemmParams p) {
+  using namespace fp4g;
+  using C = PairCfg<MX>;
+  constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES, PIECES = scale_pieces(MX), BN = 256, TILE_M = 256;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = (uint64_t*)(smem + STAGES * STAGE_BYTES);   // [STAGES] TMA landed (the leader's count both CTAs' bytes)
+  uint64_t* empty = full + STAGES;                             // [STAGES] MMAs that read the stage have finished
+  uint64_t* acc_full = empty + STAGES;                         // accumulator complete
+  uint64_t* acc_empty = acc_full + 1;                          // accumulator in registers (the leader's, by both CTAs' epilogue threads)
+  uint32_t* tmem_slot = (uint32_t*)(acc_empty + 1);
+  volatile uint32_t* abort_word = (volatile uint32_t*)(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();     // 0 = leader
+  const int worker = blockIdx.x >> 1, workers = gridDim.x >> 1;
+  const int mt = (p.M + TILE_M - 1) / TILE_M, nt = (p.N + BN - 1) / BN;
+  const int kblocks = (p.K + KB - 1) / KB, tiles = mt * nt;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 512);
+    abort_word[0] = (p.status != nullptr && *p.status != 0u) ? 0xFFu : 0u;
+    abort_word[1] = 0u;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc2(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish2();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();       // the peer's barriers are initialised, both allocations are done
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot, sf_base = tmem_base + C::ACC_COLS;
+
+  // tile t -> origin: groups of group_m row blocks x all column blocks, row block fastest, so that the pairs running
+  // together share a few rows of both operands and a group's slice of A stays in L2
+  auto tile_origin = [&](int t, int& m0, int& n0) {
+    const int per_group = p.group_m * nt;
+    const int g = t / per_group, first = g * p.group_m;
+    const int gm = min(p.group_m, mt - first);
+    const int local = t - g * per_group;
+    m0 = (first + local % gm) * TILE_M + (int)rank * 128;     // this CTA's rows of the tile
+    n0 = (local / gm) * BN;
+  };
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmAs);
+      tma_prefetch_desc(&tmW);
+      tma_prefetch_desc(&tmWs);
+      uint32_t n = 0;
+      for (int t = worker; t < tiles && *abort_word == 0u; t += workers) {
+        int m0, n0;
+        tile_origin(t, m0, n0);
+        for (int kb = 0; kb < kblocks; kb++, n++) {
+          const int s = n % STAGES;
+          if (!mbar_wait(&empty[s], ((n / STAGES) & 1) ^ 1, abort_word, SITE_EMPTY)) break;
+          uint8_t* st = smem + s * STAGE_BYTES;
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE_BYTES);
+          const uint32_t bar = mapa(smem_u32(&full[s]), 0);
+          tma_load_3d_pair(st, &tmA, bar, kb * 128, m0, 0);
+          tma_load_3d_pair(st + ROW_TILE_BYTES, &tmW, bar, kb * 128, n0 + (int)rank * 128, 0);
+          tma_load_3d_pair(st + 2 * ROW_TILE_BYTES, &tmAs, bar, 0, kb, m0 >> 7);
+          tma_load_3d_pair(st + 2 * ROW_TILE_BYTES + C::S_BYTES, &tmWs, bar, 0, kb, n0 >> 7);
+        }
+      }
+      // nothing may still be in flight into this CTA's shared memory when it exits
+      if (*abort_word != 0u && rank == 0) {
+        for (uint32_t i = (n > STAGES ? n - STAGES : 0); i < n; i++) mbar_wait_slow(&full[i % STAGES], (i / STAGES) & 1, abort_word + 1, SITE_FULL);
+      }
+    }
+  } else if (warp == 1 && rank == 0) {
+    const bool leader = elect_one();
+    constexpr uint32_t HI = desc_hi(1024), ID = idesc(MX, 256, BN);
+    const uint32_t smem16 = smem_u32(smem) >> 4;
+    uint32_t n = 0;
+    int it = 0;
+    for (int t = worker; t < tiles; t += workers, it++) {
+      if (it >= 1) {
+        if (!mbar_wait(acc_empty, (it - 1) & 1, abort_word, SITE_ACC_EMPTY)) break;
+        tc_fence_after();
+      }
+      for (int kb = 0; kb < kblocks; kb++, n++) {
+        const int s = n % STAGES;
+        if (!mbar_wait(&full[s], (n / STAGES) & 1, abort_word, SITE_FULL)) break;
+        tc_fence_after();
+        const uint32_t a = smem16 + s * (STAGE_BYTES >> 4), w = a + (ROW_TILE_BYTES >> 4), sa = w + (ROW_TILE_BYTES >> 4), sw = sa + (C::S_BYTES >> 4);
+        const uint32_t ta = sf_base + s * C::SF_COLS, tw = ta + 4 * PIECES;
+        if (leader) {
+#pragma unroll
+          for (int j = 0; j < PIECES; j++) {
+            copy_scales<2>(ta + 4 * j, sa + j * 32);
+            copy_scales<2>(tw + 8 * j, sw + j * 32);                                // columns 0-127 of the tile
+            copy_scales<2>(tw + 8 * j + 4, sw + (C::S_BYTES >> 4) + j * 32);        // columns 128-255
+          }
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const int piece = MX ? j >> 1 : j;
+            mma<MX, 2>(tmem_base, make_desc(a + j * 2, HI), make_desc(w + j * 2, HI), ID | idesc_sf(MX ? (j & 1) * 2 : 0), ta + 4 * piece, tw + 8 * piece, (kb > 0 || j > 0) ? 1u : 0u);
+          }
+          umma_commit2(mapa(smem_u32(&empty[s]), 0));
+          umma_commit2(mapa(smem_u32(&empty[s]), 1));
+        }
+        __syncwarp();
+      }
+      if (leader) {
+        umma_commit2(mapa(smem_u32(acc_full), 0));
+        umma_commit2(mapa(smem_u32(acc_full), 1));
+      }
+      __syncwarp();
+      if (*abort_word != 0u) break;
+    }
+  } else if (warp >= 4) {
+    // A thread takes one row and 128 columns into registers and hands the accumulator back before it does anything else
+    // with them: the tensor cores go on while the stores are under way.
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t src = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
+    const float alpha = tensor_scale(p);
+    int it = 0;
+    for (int t = worker; t < tiles; t += workers, it++) {
+      int m0, n0;
+      tile_origin(t, m0, n0);
+      if (!mbar_wait(acc_full, it & 1, abort_word, SITE_ACC_FULL)) break;
+      tc_fence_after();
+      uint32_t v[128];
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) tmem_ld32(src + c, v + c);
+      tmem_wait_ld();
+      tc_fence_before();
+      mbar_arrive_cluster(mapa(smem_u32(acc_empty), 0));
+      const int row = m0 + quarter * 32 + lane, col0 = n0 + half * 128;
+      if (row < p.M && col0 < p.N) pair_store(p, v, row, col0, alpha);
+    }
+  }
+
+  // nobody leaves or frees tensor memory while the peer may still read this CTA's shared memory, signal its barriers or
+  // write its accumulator
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc2(tmem_base, C::TMEM_COLS);
+  }
+  if (threadIdx.x == 0 && p.status != nullptr) {
+    const uint32_t a = *abort_word;
+    if (a != 0u && a != 0xFFu) atomicCAS(p.status, 0u, a | ((blockIdx.x & 0xFFFu) << 8));
+  }
+}
+
+// opts a kernel in to its shared memory, once a device (handles on several threads may launch at the same time)
+struct ConfiguredOnce {
+  bool done[64] = {};
+  std::mutex m;
+  template <class K>
+  cudaError_t set(K* kernel, int smem) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(m);
+    if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+    return e;
+  }
+};
+
 template <bool MX, int TN>
 static cudaError_t launch_rows_variant(const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p, int split,
                                        cudaStream_t stream) {
   using namespace fp4g;
-  static bool configured[64] = {};
-  static std::mutex configure_mutex;       // handles on several threads may launch at the same time
-  int dev = 0;
-  cudaGetDevice(&dev);
-  {
-    std::lock_guard<std::mutex> lock(configure_mutex);
-    if (dev < 0 || dev >= 64 || !configured[dev]) {
-      cudaError_t e = cudaFuncSetAttribute(gemm_fp4_rows_sm100<MX, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsCfg<MX, TN>::SMEM);
-      if (e != cudaSuccess) return e;
-      if (dev >= 0 && dev < 64) configured[dev] = true;
-    }
-  }
+  static ConfiguredOnce once;
+  cudaError_t e = once.set(gemm_fp4_rows_sm100<MX, TN>, RowsCfg<MX, TN>::SMEM);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((p.N + 127) / 128), (unsigned)((p.M + TN - 1) / TN), (unsigned)split);
   cfg.blockDim = dim3(ROWS_THREADS);
@@ -307,22 +543,55 @@ static cudaError_t launch_rows_variant(const CUtensorMap& tmA, const CUtensorMap
   return cudaLaunchKernelEx(&cfg, gemm_fp4_rows_sm100<MX, TN>, tmA, tmAs, tmW, tmWs, p);
 }
 
-Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms) {
+template <bool MX>
+static cudaError_t launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, Fp4GemmParams p, int sms,
+                                       cudaStream_t stream) {
+  using namespace fp4g;
+  static ConfiguredOnce once;
+  cudaError_t e = once.set(gemm_fp4_pair_sm100<MX>, PairCfg<MX>::SMEM);
+  if (e != cudaSuccess) return e;
+  const int mt = (p.M + 255) / 256, tiles = mt * ((p.N + 255) / 256);
+  int workers = sms / 2 < tiles ? sms / 2 : tiles;
+  const int waves = (tiles + workers - 1) / workers;
+  workers = (tiles + waves - 1) / waves;
+  // row blocks per group: 32 MB of packed A at most, groups of equal size
+  int64_t gmax = (32ll << 20) / ((int64_t)(p.K / 2 + 1) * 256);
+  if (gmax < 1) gmax = 1;
+  const int groups = (int)((mt + gmax - 1) / gmax);
+  p.group_m = (mt + groups - 1) / groups;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)workers * 2);
+  cfg.blockDim = dim3(PAIR_THREADS);
+  cfg.dynamicSmemBytes = PairCfg<MX>::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, gemm_fp4_pair_sm100<MX>, tmA, tmAs, tmW, tmWs, (const Fp4GemmParams)p);
+}
+
+Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force) {
   (void)mx;
   Fp4GemmPlan plan{};
+  plan.split = 1;
+  plan.pair = force == 2 || (force == 0 && M > 256);
+  if (plan.pair) return plan;
   plan.tn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + plan.tn - 1) / plan.tn);
   const int kblocks = (K + fp4g::KB - 1) / fp4g::KB;
   // enough CTAs to fill the SMs, at least two stages of K each
-  plan.split = 1;
   while (plan.split < 8 && tiles * plan.split * 2 <= 2 * sms && kblocks >= plan.split * 4) plan.split *= 2;
   return plan;
 }
 
 cudaError_t launch_gemm_fp4(const Fp4GemmPlan& plan, const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p,
                             int sms, cudaStream_t stream) {
-  (void)sms;
   if (p.M <= 0 || p.N <= 0 || p.K <= 0) return cudaSuccess;
+  if (plan.pair) return p.mx ? launch_pair_variant<true>(tmA, tmAs, tmW, tmWs, p, sms, stream) : launch_pair_variant<false>(tmA, tmAs, tmW, tmWs, p, sms, stream);
 #define KREA_ROWS(TN) return p.mx ? launch_rows_variant<true, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, stream) : launch_rows_variant<false, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, stream)
   switch (plan.tn) {
     case 16: KREA_ROWS(16);

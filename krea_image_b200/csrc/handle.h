@@ -55,6 +55,7 @@ struct krea_cuda {
   KreaDist* dist = nullptr;         // set by krea_cuda_dist_init
   int gemm_bn = 0;                  // GEMM tile: 0 = chosen per problem; 128 or 256 = one-CTA tile of that width,
                                     // 512 = 256 x 256 tile on a CTA pair
+  int fp4_tile = 0;                 // 4-bit GEMM: 0 = kernel chosen per problem, 1 = few-rows kernel, 2 = 256 x 256 tiles on CTA pairs
   int sm_count = 0;                 // SMs of the device (persistent kernels size their grid by it)
   void* block_ws = nullptr;         // intermediates of krea_cuda_dit_block when the caller passes no workspace
   size_t block_ws_bytes = 0;

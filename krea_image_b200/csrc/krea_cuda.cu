@@ -119,6 +119,10 @@ krea_cuda* krea_cuda_create(int device, char* err, int errlen) {
     const int v = atoi(s);
     if (v == 128 || v == 256 || v == 512) h->gemm_bn = v;     // 512: 256 x 256 tiles on CTA pairs
   }
+  if (const char* s = getenv("KREA_CUDA_FP4_TILE")) {                                     // tuning knob: kernel of the 4-bit GEMM
+    const int v = atoi(s);
+    if (v == 1 || v == 2) h->fp4_tile = v;
+  }
   if (const char* s = getenv("KREA_CUDA_EMU")) {  // tuning knob: share of exp2 evaluated on the FMA pipe (0-3 of 4)
     const int v = atoi(s);
     if (v >= 0 && v <= 1) h->emu = v;

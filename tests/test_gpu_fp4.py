@@ -1,5 +1,7 @@
 """GPU tests of the 4-bit rows (fp4_quantize, fp4_dequantize) and of the product on them (gemm_fp4) against the float64
 statement in oracle/fp4_np.py."""
+import os
+
 import numpy as np
 import pytest
 import torch
@@ -14,6 +16,21 @@ FMT = {"mx": B.FP4_MX, "nv": B.FP4_NV}
 @pytest.fixture(scope="module")
 def kc():
     k = ops.KreaCuda(0)
+    k.set_stream(torch.cuda.current_stream())
+    yield k
+    k.close()
+
+
+@pytest.fixture(scope="module", params=["by-size", "rows", "pair"])
+def kp(request):
+    """The handle of the product's tests: the kernel chosen by size, and each of the two forced on every shape."""
+    knob = {"rows": "1", "pair": "2"}.get(request.param)
+    if knob:
+        os.environ["KREA_CUDA_FP4_TILE"] = knob
+    try:
+        k = ops.KreaCuda(0)
+    finally:
+        os.environ.pop("KREA_CUDA_FP4_TILE", None)
     k.set_stream(torch.cuda.current_stream())
     yield k
     k.close()
@@ -167,7 +184,7 @@ SHAPES = [(1, 8, 1), (1, 128, 256), (1, 136, 70), (3, 64, 31), (16, 128, 512), (
 
 @pytest.mark.parametrize("fmt", ["mx", "nv"])
 @pytest.mark.parametrize("M,N,K", SHAPES)
-def test_product_sums_are_exact_where_32_bits_hold_them(kc, M, N, K, fmt):
+def test_product_sums_are_exact_where_32_bits_hold_them(kp, M, N, K, fmt):
     """Scales of 1/2, 1 and 2: every product is a multiple of 1/16 and every partial sum stays below 2^20 (K * 36 * 4), so
     that 24 bits hold them all and the result has no rounding at all; each wrong index shows."""
     rng = np.random.default_rng(M + 3 * N + 7 * K)
@@ -177,10 +194,10 @@ def test_product_sums_are_exact_where_32_bits_hold_them(kc, M, N, K, fmt):
     W, Ws, vw = _operand(qw, cw, fmt, K, 32)
     assert np.abs(va).sum(1).max() * 12 < 2 ** 20
     c = torch.full((M + 1, N + 8), -3.0, dtype=torch.float32, device="cuda")
-    n0 = kc.launches
-    kc.gemm_fp4(A, As, W, Ws, c, M, N, K, A.shape[1], W.shape[1], N + 8, FMT[fmt], epilogue=B.EPI_F32)
-    kc.wait()
-    assert kc.launches - n0 == 1
+    n0 = kp.launches
+    kp.gemm_fp4(A, As, W, Ws, c, M, N, K, A.shape[1], W.shape[1], N + 8, FMT[fmt], epilogue=B.EPI_F32)
+    kp.wait()
+    assert kp.launches - n0 == 1
     got = c.cpu().numpy()
     assert np.array_equal(got[:M, :N], (va @ vw.T).astype(np.float32))
     assert (got[M] == -3).all() and (got[:, N:] == -3).all()
@@ -194,7 +211,7 @@ def _within(got, want, bound):
 @pytest.mark.parametrize("epilogue", ["bf16", "f32", "bias_bf16", "bias_f32", "gelu", "swiglu", "resid", "resid_gate"])
 @pytest.mark.parametrize("fmt", ["mx", "nv"])
 @pytest.mark.parametrize("M,N,K", [(1, 192, 300), (40, 320, 1500), (150, 576, 520), (600, 1088, 1000)])
-def test_product_epilogues(kc, M, N, K, fmt, epilogue):
+def test_product_epilogues(kp, M, N, K, fmt, epilogue):
     rng = np.random.default_rng(M + N + K)
     qa, ca = _codes(rng, M, K, fmt, False)
     qw, cw = _codes(rng, N, K, fmt, False)
@@ -217,9 +234,9 @@ def test_product_epilogues(kc, M, N, K, fmt, epilogue):
     cols = N // 2 if epilogue == "swiglu" else N
     f32 = epilogue in ("f32", "bias_f32", "resid", "resid_gate")
     c = _dev(x0) if epilogue.startswith("resid") else torch.full((M, cols), float("nan"), dtype=torch.float32 if f32 else torch.bfloat16, device="cuda")
-    kc.gemm_fp4(A, As, W, Ws, c, M, N, K, A.shape[1], W.shape[1], cols, FMT[fmt], epilogue=kind, vec=None if epilogue in ("bf16", "f32", "gelu", "swiglu", "resid") else _dev(vec),
+    kp.gemm_fp4(A, As, W, Ws, c, M, N, K, A.shape[1], W.shape[1], cols, FMT[fmt], epilogue=kind, vec=None if epilogue in ("bf16", "f32", "gelu", "swiglu", "resid") else _dev(vec),
                 a_tensor_scale=None if ats is None else _dev(np.array([ats])), w_tensor_scale=None if wts is None else _dev(np.array([wts])))
-    kc.wait()
+    kp.wait()
     got = c.double().cpu().numpy()
     if epilogue.startswith("bias"):
         want = acc + vec
@@ -248,7 +265,7 @@ def test_product_epilogues(kc, M, N, K, fmt, epilogue):
 
 @pytest.mark.parametrize("fmt", ["mx", "nv"])
 @pytest.mark.parametrize("M,N,K", [(1, 256, 2048), (70, 264, 600), (520, 512, 768)])
-def test_product_carries_what_is_not_finite(kc, M, N, K, fmt):
+def test_product_carries_what_is_not_finite(kp, M, N, K, fmt):
     """A block scale of NaN makes its row of A (its column of C, for W) NaN and nothing else; scales past the last row are
     padding that reaches no result."""
     rng = np.random.default_rng(11)
@@ -266,8 +283,8 @@ def test_product_carries_what_is_not_finite(kc, M, N, K, fmt):
             v[fp4_np.scale_index(r, np.arange(-(-K // fp4_np.BLOCK[fmt])), fmt, K)] = nan
         t.copy_(_dev(v))
     c = torch.zeros((M, N), dtype=torch.float32, device="cuda")
-    kc.gemm_fp4(A, As, W, Ws, c, M, N, K, A.shape[1], W.shape[1], N, FMT[fmt], epilogue=B.EPI_F32)
-    kc.wait()
+    kp.gemm_fp4(A, As, W, Ws, c, M, N, K, A.shape[1], W.shape[1], N, FMT[fmt], epilogue=B.EPI_F32)
+    kp.wait()
     got = c.cpu().numpy()
     want = (np.nan_to_num(va) @ np.nan_to_num(vw).T).astype(np.float32)
     want[M // 2, :] = np.nan
