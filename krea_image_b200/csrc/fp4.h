@@ -6,7 +6,52 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 namespace krea {
+
+// Launches with programmatic stream serialisation when `pdl`: the kernel may set itself up (barriers, tensor memory) while
+// the one before it in the stream drains.  Every kernel launched through here touches memory only after griddep_wait(),
+// in every CTA, and lets its own successor start after that.  cluster: CTAs along the grid's z axis (or x when cluster_x).
+template <class... P, class... A>
+inline cudaError_t launch_kernel(void (*kernel)(P...), dim3 grid, int block, size_t smem, cudaStream_t stream, bool pdl, int cluster, bool cluster_x, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster_x ? (unsigned)cluster : 1u;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = cluster_x ? 1u : (unsigned)cluster;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// opts a kernel in to its shared memory, once a device (handles on several threads may launch at the same time)
+struct ConfiguredOnce {
+  bool done[64] = {};
+  std::mutex m;
+  template <class K>
+  cudaError_t set(K* kernel, int smem) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(m);
+    if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+    return e;
+  }
+};
 
 // rows [rows, K] of bf16 -> packed e2m1 rows + block scales.  src: row-major [rows, ld], or [K, ld] when transposed.
 struct Fp4QuantParams {
@@ -18,7 +63,7 @@ struct Fp4QuantParams {
   int64_t ld, ldq;
   int mx;                       // 1: blocks of 32, e8m0 scales; 0: blocks of 16, e4m3 scales
 };
-cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, bool transposed, cudaStream_t stream);
+cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, bool transposed, bool pdl, cudaStream_t stream);
 
 struct Fp4DequantParams {
   const uint8_t* q;
@@ -29,7 +74,7 @@ struct Fp4DequantParams {
   int64_t ldq, ldo;
   int mx;
 };
-cudaError_t launch_fp4_dequantize(const Fp4DequantParams& p, cudaStream_t stream);
+cudaError_t launch_fp4_dequantize(const Fp4DequantParams& p, bool pdl, cudaStream_t stream);
 
 struct Fp4GemmParams {
   void* C;
@@ -53,7 +98,7 @@ Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force);
 // Tensor maps: values [rows, packed row] in bytes, 128-byte swizzled boxes of 128 bytes x 128 rows (A of the few-rows kernel:
 // plan.tn rows); scales [row tile][256-value chunk][chunk] as 8-byte words, a box one chunk of one row tile (W of the pair kernel: of two)
 cudaError_t launch_gemm_fp4(const Fp4GemmPlan& plan, const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p,
-                            int sms, cudaStream_t stream);
+                            int sms, bool pdl, cudaStream_t stream);
 
 struct GatedNormParams {
   const float* x;
@@ -73,6 +118,6 @@ struct GatedNormParams {
   float x_scale, eps;
   int y_f32, out;               // out: the KREA_CUDA_OUT_* value
 };
-cudaError_t launch_gated_norm(const GatedNormParams& p, cudaStream_t stream);
+cudaError_t launch_gated_norm(const GatedNormParams& p, int sms, bool pdl, cudaStream_t stream);
 
 }  // namespace krea

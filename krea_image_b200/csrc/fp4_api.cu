@@ -47,7 +47,7 @@ int krea_cuda_fp4_quantize(krea_cuda* h, const krea_cuda_fp4_quantize_args* a) {
   p.src = (const __nv_bfloat16*)a->src; p.q = (uint8_t*)a->q; p.scales = (uint8_t*)a->scales; p.tensor_scale = a->tensor_scale;
   p.rows = a->rows; p.K = a->K; p.ld = a->ld; p.ldq = a->ldq; p.mx = a->format == KREA_CUDA_FP4_MX;
   CUDA_TRY(h, cudaSetDevice(h->device));
-  CUDA_TRY(h, launch_fp4_quantize(p, a->transposed != 0, h->stream));
+  CUDA_TRY(h, launch_fp4_quantize(p, a->transposed != 0, h->pdl, h->stream));
   h->launches++;
   return KREA_CUDA_OK;
 }
@@ -60,7 +60,7 @@ int krea_cuda_fp4_dequantize(krea_cuda* h, const krea_cuda_fp4_dequantize_args* 
   p.q = (const uint8_t*)a->q; p.scales = (const uint8_t*)a->scales; p.tensor_scale = a->tensor_scale; p.out = (__nv_bfloat16*)a->out;
   p.rows = a->rows; p.K = a->K; p.ldq = a->ldq; p.ldo = a->ldo; p.mx = a->format == KREA_CUDA_FP4_MX;
   CUDA_TRY(h, cudaSetDevice(h->device));
-  CUDA_TRY(h, launch_fp4_dequantize(p, h->stream));
+  CUDA_TRY(h, launch_fp4_dequantize(p, h->pdl, h->stream));
   h->launches++;
   return KREA_CUDA_OK;
 }
@@ -90,7 +90,7 @@ int krea_cuda_gemm_fp4(krea_cuda* h, const krea_cuda_gemm_fp4_args* a) {
   p.vec = uses_vec ? a->vec : nullptr;
   p.a_ts = a->a_tensor_scale; p.w_ts = a->w_tensor_scale;
   p.status = h->status_dev;
-  CUDA_TRY(h, launch_gemm_fp4(plan, tmA, tmAs, tmW, tmWs, p, h->sm_count, h->stream));
+  CUDA_TRY(h, launch_gemm_fp4(plan, tmA, tmAs, tmW, tmWs, p, h->sm_count, h->pdl, h->stream));
   h->launches++;
   return KREA_CUDA_OK;
 }
@@ -105,7 +105,7 @@ int krea_cuda_gated_norm(krea_cuda* h, const krea_cuda_gated_norm_args* a) {
   p.rows = a->rows; p.width = a->width; p.ld_x = a->ld_x; p.ld_y = a->ld_y; p.ld_xo = a->ld_xo; p.ld_h = a->ld_h;
   p.mod_rows = a->mod_rows; p.mod_ld = a->mod_ld; p.x_scale = a->x_scale; p.eps = a->eps; p.y_f32 = a->y_f32 != 0; p.out = a->out;
   CUDA_TRY(h, cudaSetDevice(h->device));
-  CUDA_TRY(h, launch_gated_norm(p, h->stream));
+  CUDA_TRY(h, launch_gated_norm(p, h->sm_count, h->pdl, h->stream));
   h->launches++;
   return KREA_CUDA_OK;
 }

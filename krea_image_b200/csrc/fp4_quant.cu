@@ -42,33 +42,45 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_quantize_rows_kernel(const Fp4
   constexpr int RUNS = MX ? 32 : 16;             // warp items that cover the 128 rows of a scale tile
   const int64_t chunks = (p.K + 255) / 256;
   const int groups = (int)chunks * (256 / GROUP);
-  const int64_t items = (int64_t)((p.rows + 127) / 128) * RUNS * groups;
+  const int64_t items = (int64_t)((p.rows + 127) / 128) * RUNS * (groups / 2);          // two groups at a time
   const int lane = threadIdx.x & 31, in_row = lane % LANES, rr = lane / LANES;
-  const float ts = MX || !p.tensor_scale ? 1.f : __ldg(p.tensor_scale);
-  const float inv6 = MX ? 1.f : 1.f / (6.f * ts);
+  griddep_wait();
+  griddep_launch();
+  __shared__ NvTable nv;
+  if constexpr (!MX) {
+    if (threadIdx.x < 128) nv_table_fill(nv, p.tensor_scale ? __ldg(p.tensor_scale) : 1.f, threadIdx.x);
+    __syncthreads();
+  }
   const int64_t step = (int64_t)gridDim.x * (FQ_THREADS / 32);
   for (int64_t it = (int64_t)blockIdx.x * (FQ_THREADS / 32) + (threadIdx.x >> 5); it < items; it += step) {
-    const int g = (int)(it % groups);
-    const int64_t tr = it / groups;
+    const int g = (int)(it % (groups / 2)) * 2;
+    const int64_t tr = it / (groups / 2);
     const int run = (int)(tr % RUNS);
     const int row = (int)(tr / RUNS) * 128 + (rr & 3) * 32 + (MX ? run : run * 2 + (rr >> 2));
-    const int k0 = g * GROUP + in_row * 16;
-    uint32_t w[8];
-    load16(p.src + (int64_t)row * p.ld + k0, row < p.rows ? p.K - k0 : 0, w);
-    uint32_t amax = amax_bits<8>(w), code;
-    uint2 out;
-    if constexpr (MX) {
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      code = mx_scale_code(amax);
-      out = make_uint2(mx_encode8(w, code), mx_encode8(w + 4, code));
-    } else {
-      code = nv_scale_code(amax, ts, inv6);
-      const NvBorders b = nv_borders(code, ts);
-      out = make_uint2(nv_encode8(w, code, b), nv_encode8(w + 4, code, b));
+    const __nv_bfloat16* src = p.src + (int64_t)row * p.ld;
+    uint32_t w[2][8];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {                // both loads are under way before the first is used
+      const int k0 = (g + i) * GROUP + in_row * 16;
+      load16(src + k0, row < p.rows ? p.K - k0 : 0, w[i]);
     }
-    if (row < p.rows && k0 < ((p.K + 31) & ~31)) *(uint2*)(p.q + (int64_t)row * p.ldq + (k0 >> 1)) = out;
-    const int block = MX ? k0 >> 5 : k0 >> 4;
-    if (!MX || (lane & 1) == 0) p.scales[scale_offset<MX>(row, block, chunks)] = (uint8_t)code;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int k0 = (g + i) * GROUP + in_row * 16;
+      uint32_t amax = amax_bits<8>(w[i]), code, out[2];
+      if constexpr (MX) {
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        code = mx_scale_code(amax);
+        out[0] = mx_encode8(w[i], code);
+        out[1] = mx_encode8(w[i] + 4, code);
+      } else {
+        code = nv_scale_code(amax, nv);
+        nv_encode<8>(w[i], code, nv, out);
+      }
+      if (row < p.rows && k0 < ((p.K + 31) & ~31)) *(uint2*)(p.q + (int64_t)row * p.ldq + (k0 >> 1)) = make_uint2(out[0], out[1]);
+      const int block = MX ? k0 >> 5 : k0 >> 4;
+      if (!MX || (lane & 1) == 0) p.scales[scale_offset<MX>(row, block, chunks)] = (uint8_t)code;
+    }
   }
 }
 
@@ -82,6 +94,10 @@ __global__ void __launch_bounds__(FT_THREADS) fp4_quantize_cols_kernel(const Fp4
   const int64_t chunks = (p.K + 255) / 256;
   const int n0 = blockIdx.x * FT_N, k0 = blockIdx.y * FT_K;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  griddep_wait();
+  griddep_launch();
+  __shared__ NvTable nv;
+  if constexpr (!MX) nv_table_fill(nv, p.tensor_scale ? __ldg(p.tensor_scale) : 1.f, threadIdx.x);
   for (int i = threadIdx.x; i < FT_K * (FT_N / 8); i += FT_THREADS) {
     const int kr = i / (FT_N / 8), c = (i % (FT_N / 8)) * 8;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -103,8 +119,6 @@ __global__ void __launch_bounds__(FT_THREADS) fp4_quantize_cols_kernel(const Fp4
     *(uint4*)&tile[kr][c >> 1] = v;
   }
   __syncthreads();
-  const float ts = MX || !p.tensor_scale ? 1.f : __ldg(p.tensor_scale);
-  const float inv6 = MX ? 1.f : 1.f / (6.f * ts);
   uint32_t t[32];
 #pragma unroll
   for (int i = 0; i < 32; i++) t[i] = tile[warp * 32 + i][lane];
@@ -123,10 +137,8 @@ __global__ void __launch_bounds__(FT_THREADS) fp4_quantize_cols_kernel(const Fp4
     } else {
 #pragma unroll
       for (int blk = 0; blk < 2; blk++) {
-        const uint32_t code = nv_scale_code(amax_bits<8>(w + 8 * blk), ts, inv6);
-        const NvBorders b = nv_borders(code, ts);
-        out[2 * blk] = nv_encode8(w + 8 * blk, code, b);
-        out[2 * blk + 1] = nv_encode8(w + 8 * blk + 4, code, b);
+        const uint32_t code = nv_scale_code(amax_bits<8>(w + 8 * blk), nv);
+        nv_encode<8>(w + 8 * blk, code, nv, out + 2 * blk);
         p.scales[scale_offset<MX>(n, (kb >> 4) + blk, chunks)] = (uint8_t)code;
       }
     }
@@ -139,21 +151,17 @@ __global__ void __launch_bounds__(FT_THREADS) fp4_quantize_cols_kernel(const Fp4
   }
 }
 
-cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, bool transposed, cudaStream_t stream) {
+cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, bool transposed, bool pdl, cudaStream_t stream) {
   if (p.rows <= 0 || p.K <= 0) return cudaSuccess;
   const int64_t tiles = (p.rows + 127) / 128, chunks = (p.K + 255) / 256;
   if (transposed) {
     const dim3 grid((unsigned)(tiles * (128 / FT_N)), (unsigned)(chunks * (256 / FT_K)));      // padding included: its scales are written too
-    if (p.mx) fp4_quantize_cols_kernel<true><<<grid, FT_THREADS, 0, stream>>>(p);
-    else fp4_quantize_cols_kernel<false><<<grid, FT_THREADS, 0, stream>>>(p);
-    return cudaGetLastError();
+    return launch_kernel(p.mx ? fp4_quantize_cols_kernel<true> : fp4_quantize_cols_kernel<false>, grid, FT_THREADS, 0, stream, pdl, 1, false, p);
   }
-  const int64_t items = tiles * (p.mx ? 32 * 2 : 16 * 4) * chunks;
+  const int64_t items = tiles * (p.mx ? 32 * 1 : 16 * 2) * chunks;
   int64_t blocks = (items + FQ_THREADS / 32 - 1) / (FQ_THREADS / 32);
-  if (blocks > 148 * 64) blocks = 148 * 64;
-  if (p.mx) fp4_quantize_rows_kernel<true><<<(unsigned)blocks, FQ_THREADS, 0, stream>>>(p);
-  else fp4_quantize_rows_kernel<false><<<(unsigned)blocks, FQ_THREADS, 0, stream>>>(p);
-  return cudaGetLastError();
+  if (blocks > 148 * 16) blocks = 148 * 16;          // about two rounds of resident CTAs: each fills its table once
+  return launch_kernel(p.mx ? fp4_quantize_rows_kernel<true> : fp4_quantize_rows_kernel<false>, dim3((unsigned)blocks), FQ_THREADS, 0, stream, pdl, 1, false, p);
 }
 
 // ---- back to bf16: bf16(e2m1 * block scale * tensor scale), rounded once from f32 ----
@@ -168,6 +176,8 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_dequantize_kernel(const Fp4Deq
   const int64_t chunks = (p.K + 255) / 256;
   const int per_row = (p.K + 15) / 16;                 // 16 values a thread
   const int64_t items = (int64_t)p.rows * per_row, step = (int64_t)gridDim.x * FQ_THREADS;
+  griddep_wait();
+  griddep_launch();
   const float ts = MX || !p.tensor_scale ? 1.f : __ldg(p.tensor_scale);
   for (int64_t it = (int64_t)blockIdx.x * FQ_THREADS + threadIdx.x; it < items; it += step) {
     const int row = (int)(it / per_row), k0 = (int)(it - (int64_t)row * per_row) * 16;
@@ -196,14 +206,12 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_dequantize_kernel(const Fp4Deq
   }
 }
 
-cudaError_t launch_fp4_dequantize(const Fp4DequantParams& p, cudaStream_t stream) {
+cudaError_t launch_fp4_dequantize(const Fp4DequantParams& p, bool pdl, cudaStream_t stream) {
   if (p.rows <= 0 || p.K <= 0) return cudaSuccess;
   const int64_t items = (int64_t)p.rows * ((p.K + 15) / 16);
   int64_t blocks = (items + FQ_THREADS - 1) / FQ_THREADS;
   if (blocks > 148 * 64) blocks = 148 * 64;
-  if (p.mx) fp4_dequantize_kernel<true><<<(unsigned)blocks, FQ_THREADS, 0, stream>>>(p);
-  else fp4_dequantize_kernel<false><<<(unsigned)blocks, FQ_THREADS, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_kernel(p.mx ? fp4_dequantize_kernel<true> : fp4_dequantize_kernel<false>, dim3((unsigned)blocks), FQ_THREADS, 0, stream, pdl, 1, false, p);
 }
 
 }  // namespace krea

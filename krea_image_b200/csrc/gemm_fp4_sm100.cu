@@ -16,8 +16,6 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <mutex>
-
 #include "../../include/krea_cuda.h"
 #include "fp4.h"
 #include "sm100_pair.cuh"
@@ -184,13 +182,16 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int kb0 = (int)((int64_t)kblocks * rank / split), kb1 = (int)((int64_t)kblocks * (rank + 1) / split);
 
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmWs);
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmAs);
     for (int s = 0; s < STAGES; s++) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
-    abort_word[0] = (p.status != nullptr && *p.status != 0u) ? 0xFFu : 0u;
-    abort_word[1] = 0u;
+    abort_word[0] = abort_word[1] = 0u;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -201,13 +202,12 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot, sf_base = tmem_base + C::ACC_COLS;
+  griddep_wait();
+  griddep_launch();
 
   if (warp == 0) {
     if (lane == 0) {
-      tma_prefetch_desc(&tmW);
-      tma_prefetch_desc(&tmWs);
-      tma_prefetch_desc(&tmA);
-      tma_prefetch_desc(&tmAs);
+      if (p.status != nullptr && *(volatile uint32_t*)p.status != 0u) abort_word[0] = 0xFFu;      // an earlier kernel gave up: do nothing
       uint32_t n = 0;
       for (int kb = kb0; kb < kb1 && *abort_word == 0u; kb++, n++) {
         const int s = n % STAGES;
@@ -368,14 +368,17 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int kblocks = (p.K + KB - 1) / KB, tiles = mt * nt;
 
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmWs);
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmAs);
     for (int s = 0; s < STAGES; s++) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 512);
-    abort_word[0] = (p.status != nullptr && *p.status != 0u) ? 0xFFu : 0u;
-    abort_word[1] = 0u;
+    abort_word[0] = abort_word[1] = 0u;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -390,6 +393,8 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 
   // tile t -> origin: groups of group_m row blocks x all column blocks, row block fastest, so that the pairs running
   // together share a few rows of both operands and a group's slice of A stays in L2
+  griddep_wait();
+  griddep_launch();
   auto tile_origin = [&](int t, int& m0, int& n0) {
     const int per_group = p.group_m * nt;
     const int g = t / per_group, first = g * p.group_m;
@@ -400,10 +405,7 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   };
   if (warp == 0) {
     if (lane == 0) {
-      tma_prefetch_desc(&tmA);
-      tma_prefetch_desc(&tmAs);
-      tma_prefetch_desc(&tmW);
-      tma_prefetch_desc(&tmWs);
+      if (p.status != nullptr && *(volatile uint32_t*)p.status != 0u) abort_word[0] = 0xFFu;      // an earlier kernel gave up: do nothing
       uint32_t n = 0;
       for (int t = worker; t < tiles && *abort_word == 0u; t += workers) {
         int m0, n0;
@@ -505,46 +507,19 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
 }
 
-// opts a kernel in to its shared memory, once a device (handles on several threads may launch at the same time)
-struct ConfiguredOnce {
-  bool done[64] = {};
-  std::mutex m;
-  template <class K>
-  cudaError_t set(K* kernel, int smem) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    std::lock_guard<std::mutex> lock(m);
-    if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
-    return e;
-  }
-};
-
 template <bool MX, int TN>
-static cudaError_t launch_rows_variant(const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p, int split,
+static cudaError_t launch_rows_variant(const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p, int split, bool pdl,
                                        cudaStream_t stream) {
   using namespace fp4g;
   static ConfiguredOnce once;
   cudaError_t e = once.set(gemm_fp4_rows_sm100<MX, TN>, RowsCfg<MX, TN>::SMEM);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.N + 127) / 128), (unsigned)((p.M + TN - 1) / TN), (unsigned)split);
-  cfg.blockDim = dim3(ROWS_THREADS);
-  cfg.dynamicSmemBytes = RowsCfg<MX, TN>::SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = (unsigned)split;
-  cfg.attrs = attr;
-  cfg.numAttrs = split > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, gemm_fp4_rows_sm100<MX, TN>, tmA, tmAs, tmW, tmWs, p);
+  const dim3 grid((unsigned)((p.N + 127) / 128), (unsigned)((p.M + TN - 1) / TN), (unsigned)split);
+  return launch_kernel(gemm_fp4_rows_sm100<MX, TN>, grid, ROWS_THREADS, RowsCfg<MX, TN>::SMEM, stream, pdl, split, false, tmA, tmAs, tmW, tmWs, p);
 }
 
 template <bool MX>
-static cudaError_t launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, Fp4GemmParams p, int sms,
+static cudaError_t launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, Fp4GemmParams p, int sms, bool pdl,
                                        cudaStream_t stream) {
   using namespace fp4g;
   static ConfiguredOnce once;
@@ -559,19 +534,7 @@ static cudaError_t launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap
   if (gmax < 1) gmax = 1;
   const int groups = (int)((mt + gmax - 1) / gmax);
   p.group_m = (mt + groups - 1) / groups;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)workers * 2);
-  cfg.blockDim = dim3(PAIR_THREADS);
-  cfg.dynamicSmemBytes = PairCfg<MX>::SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, gemm_fp4_pair_sm100<MX>, tmA, tmAs, tmW, tmWs, (const Fp4GemmParams)p);
+  return launch_kernel(gemm_fp4_pair_sm100<MX>, dim3((unsigned)workers * 2), PAIR_THREADS, PairCfg<MX>::SMEM, stream, pdl, 2, true, tmA, tmAs, tmW, tmWs, p);
 }
 
 Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force) {
@@ -589,10 +552,10 @@ Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force) {
 }
 
 cudaError_t launch_gemm_fp4(const Fp4GemmPlan& plan, const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p,
-                            int sms, cudaStream_t stream) {
+                            int sms, bool pdl, cudaStream_t stream) {
   if (p.M <= 0 || p.N <= 0 || p.K <= 0) return cudaSuccess;
-  if (plan.pair) return p.mx ? launch_pair_variant<true>(tmA, tmAs, tmW, tmWs, p, sms, stream) : launch_pair_variant<false>(tmA, tmAs, tmW, tmWs, p, sms, stream);
-#define KREA_ROWS(TN) return p.mx ? launch_rows_variant<true, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, stream) : launch_rows_variant<false, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, stream)
+  if (plan.pair) return p.mx ? launch_pair_variant<true>(tmA, tmAs, tmW, tmWs, p, sms, pdl, stream) : launch_pair_variant<false>(tmA, tmAs, tmW, tmWs, p, sms, pdl, stream);
+#define KREA_ROWS(TN) return p.mx ? launch_rows_variant<true, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, pdl, stream) : launch_rows_variant<false, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, pdl, stream)
   switch (plan.tn) {
     case 16: KREA_ROWS(16);
     case 32: KREA_ROWS(32);

@@ -40,7 +40,7 @@ struct krea_cuda {
   int emu = 0;                      // 1: one of every 4 element pairs takes the polynomial exp2
   int persist = 1;                  // persistent attention kernel (one CTA per SM walking over the work items):
                                     // 0 never, 1 when there are more items than SMs, 2 always
-  bool pdl = true;                  // fused call: pre-pass and attention use programmatic dependent launch
+  bool pdl = true;                  // fused call, 4-bit operators and gated norm: programmatic dependent launch
   bool q_tma = true;                // plain attention operator: Q tiles arrive as TMA loads
   bool o_tma = true;                // attention output tiles leave shared memory as TMA stores
   bool static_bound = true;         // let the fused call replace the running max by the QK-norm logit bound
