@@ -96,8 +96,9 @@ struct Fp4GemmPlan {
 // force: 0 = choose by size, 1 = few-rows kernel, 2 = CTA pairs
 Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force);
 // Tensor maps: values [rows, packed row] in bytes, 128-byte swizzled boxes of 128 bytes x 128 rows (A of the few-rows kernel:
-// plan.tn rows); scales [row tile][256-value chunk][chunk] as 8-byte words, a box one chunk of one row tile (W of the pair kernel: of two)
-cudaError_t launch_gemm_fp4(const Fp4GemmPlan& plan, const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p,
+// plan.tn rows); scales [row tile][256-value chunk][chunk] as 8-byte words, a box one chunk of one row tile (W of the pair kernel: of two);
+// C of the pair kernel (not with RESID_GATE): boxes of 32 rows x 128 bytes, 128-byte swizzled
+cudaError_t launch_gemm_fp4(const Fp4GemmPlan& plan, const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const CUtensorMap& tmC, const Fp4GemmParams& p,
                             int sms, bool pdl, cudaStream_t stream);
 
 struct GatedNormParams {

@@ -33,6 +33,18 @@ static int make_scales_map(krea_cuda* h, CUtensorMap* tm, const void* base, int 
   if (r != CUDA_SUCCESS) return fail(h, KREA_CUDA_E_CUDA, "gemm_fp4: cuTensorMapEncodeTiled(%s) failed with %d", what, (int)r);
   return KREA_CUDA_OK;
 }
+// C in boxes of 32 rows x 128 bytes, 128-byte swizzle; what a box has outside is not written
+static int make_out_map(krea_cuda* h, CUtensorMap* tm, void* base, int rows, int cols, int64_t ld, bool f32) {
+  const int es = f32 ? 4 : 2;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
+  cuuint64_t strides[2] = {(cuuint64_t)ld * es, (cuuint64_t)ld * es * (cuuint64_t)rows};
+  cuuint32_t box[3] = {(cuuint32_t)(128 / es), 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = h->encode(tm, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(h, KREA_CUDA_E_CUDA, "gemm_fp4: cuTensorMapEncodeTiled(C) failed with %d", (int)r);
+  return KREA_CUDA_OK;
+}
 
 extern "C" {
 
@@ -78,19 +90,21 @@ int krea_cuda_gemm_fp4(krea_cuda* h, const krea_cuda_gemm_fp4_args* a) {
   }
   const bool mx = a->format == KREA_CUDA_FP4_MX;
   const Fp4GemmPlan plan = plan_gemm_fp4(a->M, a->N, a->K, mx, h->sm_count, h->fp4_tile);
-  CUtensorMap tmA, tmAs, tmW, tmWs;
+  CUtensorMap tmA, tmAs, tmW, tmWs, tmC;
+  memset(&tmC, 0, sizeof(tmC));
   int rc;
   if ((rc = make_values_map(h, &tmA, a->A, a->M, a->K, a->lda, plan.pair ? 128 : plan.tn, "A"))) return rc;
   if ((rc = make_values_map(h, &tmW, a->W, a->N, a->K, a->ldw, 128, "W"))) return rc;
   if ((rc = make_scales_map(h, &tmAs, a->a_scales, a->format, a->M, a->K, 1, "a_scales"))) return rc;
   if ((rc = make_scales_map(h, &tmWs, a->w_scales, a->format, a->N, a->K, plan.pair ? 2 : 1, "w_scales"))) return rc;
+  if (plan.pair && (rc = make_out_map(h, &tmC, a->C, a->M, a->epilogue == KREA_CUDA_EPI_SWIGLU ? a->N / 2 : a->N, a->ldc, epilogue_f32(a->epilogue)))) return rc;
   Fp4GemmParams p{};
   p.C = a->C; p.ldc = a->ldc; p.M = a->M; p.N = a->N; p.K = a->K; p.epi = a->epilogue; p.mx = mx;
   const bool uses_vec = a->epilogue == KREA_CUDA_EPI_RESID_GATE || a->epilogue == KREA_CUDA_EPI_BIAS_BF16 || a->epilogue == KREA_CUDA_EPI_BIAS_F32;
   p.vec = uses_vec ? a->vec : nullptr;
   p.a_ts = a->a_tensor_scale; p.w_ts = a->w_tensor_scale;
   p.status = h->status_dev;
-  CUDA_TRY(h, launch_gemm_fp4(plan, tmA, tmAs, tmW, tmWs, p, h->sm_count, h->pdl, h->stream));
+  CUDA_TRY(h, launch_gemm_fp4(plan, tmA, tmAs, tmW, tmWs, tmC, p, h->sm_count, h->pdl, h->stream));
   h->launches++;
   return KREA_CUDA_OK;
 }

@@ -45,7 +45,6 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_quantize_rows_kernel(const Fp4
   const int64_t items = (int64_t)((p.rows + 127) / 128) * RUNS * (groups / 2);          // two groups at a time
   const int lane = threadIdx.x & 31, in_row = lane % LANES, rr = lane / LANES;
   griddep_wait();
-  griddep_launch();
   __shared__ NvTable nv;
   if constexpr (!MX) {
     if (threadIdx.x < 128) nv_table_fill(nv, p.tensor_scale ? __ldg(p.tensor_scale) : 1.f, threadIdx.x);
@@ -95,7 +94,6 @@ __global__ void __launch_bounds__(FT_THREADS) fp4_quantize_cols_kernel(const Fp4
   const int n0 = blockIdx.x * FT_N, k0 = blockIdx.y * FT_K;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
-  griddep_launch();
   __shared__ NvTable nv;
   if constexpr (!MX) nv_table_fill(nv, p.tensor_scale ? __ldg(p.tensor_scale) : 1.f, threadIdx.x);
   for (int i = threadIdx.x; i < FT_K * (FT_N / 8); i += FT_THREADS) {
@@ -177,7 +175,6 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_dequantize_kernel(const Fp4Deq
   const int per_row = (p.K + 15) / 16;                 // 16 values a thread
   const int64_t items = (int64_t)p.rows * per_row, step = (int64_t)gridDim.x * FQ_THREADS;
   griddep_wait();
-  griddep_launch();
   const float ts = MX || !p.tensor_scale ? 1.f : __ldg(p.tensor_scale);
   for (int64_t it = (int64_t)blockIdx.x * FQ_THREADS + threadIdx.x; it < items; it += step) {
     const int row = (int)(it / per_row), k0 = (int)(it - (int64_t)row * per_row) * 16;

@@ -150,7 +150,6 @@ __global__ void __maxnreg__(REGS) gated_norm_kernel(const GatedNormParams p) {
   __shared__ float part[2][2][32];        // [row parity][which sum][warp]
   __shared__ NvTable nv;
   griddep_wait();
-  griddep_launch();
   const int t = threadIdx.x;
   unsigned row = blockIdx.x;                 // unsigned: row + gridDim.x passes 2^31 at the end of the longest inputs
   RowPieces<HOLD, Y32> in;
@@ -214,6 +213,7 @@ __global__ void __maxnreg__(REGS) gated_norm_kernel(const GatedNormParams p) {
     const int now = (int)row;
     row += gridDim.x;
     if (row < (unsigned)p.rows) in.template fetch<V8>(p, (int)row);
+    else griddep_launch();       // not before the last row: a successor that waits on the SM would take L1 away
     if (!p.h) continue;
     if constexpr (AHEAD) {
 #pragma unroll
@@ -295,6 +295,9 @@ cudaError_t launch_gated_norm(const GatedNormParams& p, int sms, bool pdl, cudaS
   const uintptr_t vec32 = (uintptr_t)p.post | (uintptr_t)p.gate | (uintptr_t)p.mul | (uintptr_t)p.add | (uintptr_t)(p.mod_rows > 0 ? p.mod_ld * 4 : 0);
   const bool v8 = ((rows32 | vec32) & 31u) == 0;
   if (p.rows < 2 * sms && padded <= 8192) return launch_rows<1, 64, true, false>(p, threads(1), sms, pdl, stream);
+  // Not programmatic: CTAs that start on an SM as the kernel before leaves it keep that kernel's split of L1 and shared memory,
+  // and after a GEMM the vectors have no L1 to stay in (norm + 4-bit product at 4608 x 6144: 154 us against 135)
+  pdl = false;
   if (padded <= 16384) return v8 ? launch_rows<2, 64, false, true>(p, threads(2), sms, pdl, stream) : launch_rows<2, 64, false, false>(p, threads(2), sms, pdl, stream);
   return launch_rows<4, 64, false, false>(p, threads(4), sms, pdl, stream);
 }

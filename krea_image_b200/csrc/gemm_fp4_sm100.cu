@@ -97,46 +97,94 @@ __device__ __forceinline__ void finish8(const Fp4GemmParams& p, float* f, int ro
   }
 }
 
-// Epilogue of a thread of the pair kernel: columns [col0, col0 + 128) of one row of C, as far as N goes (N a multiple of 8,
-// of 64 with SwiGLU).
-__device__ __forceinline__ void pair_store(const Fp4GemmParams& p, const uint32_t* v, int row, int col0, float alpha) {
-  const int left = p.N - col0;
-  if (p.epi == KREA_CUDA_EPI_SWIGLU) {
-    __nv_bfloat16* o = (__nv_bfloat16*)p.C + (int64_t)row * p.ldc + (col0 >> 1);
+// Epilogue of a warp of the pair kernel: rows [row0, row0 + 32), a lane each, columns [col0, col0 + 128).  The results leave
+// through shared memory as boxes of 32 rows x 128 bytes by TMA, which writes whole lines and stops at the last row and
+// column by itself.  Stored from registers, 32 bytes of 32 rows at a time, a tile took 5000 clocks and held up the loads of
+// the next one (3800 clocks a tile lost at 4608 x 15360 x 6144).  box: one box, used again and again, or `many` in a row.
+__device__ __forceinline__ void pair_store(const Fp4GemmParams& p, const CUtensorMap& tmC, const uint32_t* v, int row0, int col0, float alpha, uint8_t* box, bool many, int lane) {
+  const bool swiglu = p.epi == KREA_CUDA_EPI_SWIGLU, f32 = p.epi == KREA_CUDA_EPI_F32 || p.epi == KREA_CUDA_EPI_BIAS_F32;
+  uint32_t dst = smem_u32(box) + lane * 128;
+  // 16 bytes at place q of the lane's row, swizzled as the tensor map has it
+  const auto put = [&](int q, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t)((q ^ (lane & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+  };
+  const auto acc = [&](int i) { return __uint_as_float(v[i]) * alpha; };
+  const auto begin = [&] {                       // the box before this one has been read
+    if (many) return;
+    if (lane == 0) tma_store_wait_read();
+    __syncwarp();
+  };
+  const auto send = [&](int col) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(&tmC, box, col, row0, 0);
+      tma_store_commit();
+    }
+    if (many) {
+      box += 32 * 128;
+      dst += 32 * 128;
+    }
+  };
+  if (swiglu) {                                  // 32 gate columns, then the 32 they gate: 64 columns of C
+    begin();
 #pragma unroll
-    for (int c = 0; c < 128; c += 64) {
-      if (c >= left) break;
-      uint32_t pk[16];
+    for (int q = 0; q < 8; q++) {
+      uint32_t pk[4];
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const float g0 = __uint_as_float(v[c + 2 * e]) * alpha, g1 = __uint_as_float(v[c + 2 * e + 1]) * alpha;
-        const float u0 = __uint_as_float(v[c + 32 + 2 * e]) * alpha, u1 = __uint_as_float(v[c + 33 + 2 * e]) * alpha;
-        pk[e] = pack_bf16x2(g0 * sigmoid_approx(g0) * u0, g1 * sigmoid_approx(g1) * u1);
+      for (int e = 0; e < 4; e++) {
+        const int c = (q >> 2) * 64 + (q & 3) * 8 + 2 * e;
+        const float g0 = acc(c), g1 = acc(c + 1);
+        pk[e] = pack_bf16x2(g0 * sigmoid_approx(g0) * acc(c + 32), g1 * sigmoid_approx(g1) * acc(c + 33));
       }
-      if ((((uintptr_t)(o + (c >> 1))) & 31u) == 0) {
-        st_global_32B(o + (c >> 1), pk);
-        st_global_32B(o + (c >> 1) + 16, pk + 8);
-      } else {
+      put(q, pk[0], pk[1], pk[2], pk[3]);
+    }
+    send(col0 >> 1);
+    return;
+  }
+  if (f32) {
 #pragma unroll
-        for (int q = 0; q < 4; q++) *(uint4*)(o + (c >> 1) + q * 8) = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+    for (int c0 = 0; c0 < 128; c0 += 32) {
+      if (col0 + c0 >= p.N) break;
+      begin();
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        const int c = c0 + q * 4;
+        float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p.epi == KREA_CUDA_EPI_BIAS_F32 && col0 + c < p.N) b = __ldg((const float4*)(p.vec + col0 + c));
+        put(q, __float_as_uint(acc(c) + b.x), __float_as_uint(acc(c + 1) + b.y), __float_as_uint(acc(c + 2) + b.z), __float_as_uint(acc(c + 3) + b.w));
       }
+      send(col0 + c0);
     }
     return;
   }
-  if (p.epi == KREA_CUDA_EPI_BF16 && left >= 128 && (((uintptr_t)p.C | (uintptr_t)(p.ldc * 2)) & 31u) == 0) {
-    __nv_bfloat16* o = (__nv_bfloat16*)p.C + (int64_t)row * p.ldc + col0;
 #pragma unroll
-    for (int c = 0; c < 128; c += 16) {
-      uint32_t pk[8];
+  for (int c0 = 0; c0 < 128; c0 += 64) {
+    if (col0 + c0 >= p.N) break;
+    begin();
 #pragma unroll
-      for (int e = 0; e < 8; e++) pk[e] = pack_bf16x2(__uint_as_float(v[c + 2 * e]) * alpha, __uint_as_float(v[c + 2 * e + 1]) * alpha);
-      st_global_32B(o + c, pk);
+    for (int q = 0; q < 8; q++) {
+      const int c = c0 + q * 8;
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[e] = acc(c + e);
+      if (p.epi == KREA_CUDA_EPI_BIAS_BF16 && col0 + c < p.N) {
+        const float4 a = __ldg((const float4*)(p.vec + col0 + c)), b = __ldg((const float4*)(p.vec + col0 + c) + 1);
+        f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+      } else if (p.epi == KREA_CUDA_EPI_GELU) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = gelu_tanh(f[e]);
+      }
+      put(q, pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
     }
-    return;
+    send(col0 + c0);
   }
+}
+// C (f32) += vec * acc for 128 columns of a row
+__device__ __forceinline__ void pair_add(const Fp4GemmParams& p, const uint32_t* v, int row, int col0, float alpha) {
 #pragma unroll
   for (int c = 0; c < 128; c += 8) {
-    if (c >= left) break;
+    if (col0 + c >= p.N) break;
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) f[e] = __uint_as_float(v[c + e]) * alpha;
@@ -335,11 +383,13 @@ struct PairCfg {
   static constexpr int S_BYTES = scale_chunk(MX);
   // this CTA's 128 rows of A and of W (half of the tile's columns), the scales of its rows of A and of all 256 columns
   static constexpr int STAGE_BYTES = 2 * ROW_TILE_BYTES + 3 * S_BYTES;
-  static constexpr int STAGES = MX ? 6 : 5;
+  static constexpr int STAGES = 5;
+  static constexpr int OUT_BYTES = 32 * 128;               // a warp's output box: 32 rows x 128 bytes
   static constexpr int SF_COLS = 3 * 4 * scale_pieces(MX);
   static constexpr int ACC_COLS = 256;
   static constexpr int TMEM_COLS = 512;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 256 + 1024;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 8 * OUT_BYTES + 256 + 1024;
+  static_assert(8 * 4 * OUT_BYTES <= STAGES * STAGE_BYTES, "the last tile's boxes lie over the stages");
   static_assert(ACC_COLS + STAGES * SF_COLS <= TMEM_COLS && SMEM <= 227 * 1024, "tile does not fit");
 };
 constexpr int PAIR_THREADS = 384;   // warp 0 TMA, warp 1 MMA, warps 4-11 epilogue (two for each quarter of the tensor-memory lanes)
@@ -348,16 +398,17 @@ constexpr int PAIR_THREADS = 384;   // warp 0 TMA, warp 1 MMA, warps 4-11 epilog
 template <bool MX>
 __global__ void __launch_bounds__(fp4g::PAIR_THREADS, 1)
 gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs, const __grid_constant__ CUtensorMap tmW,
-                    const __grid_constant__ CUtensorMap tmWs, const Fp4GemmParams p) {
+                    const __grid_constant__ CUtensorMap tmWs, const __grid_constant__ CUtensorMap tmC, const Fp4GemmParams p) {
   using namespace fp4g;
   using C = PairCfg<MX>;
   constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES, PIECES = scale_pieces(MX), BN = 256, TILE_M = 256;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t* full = (uint64_t*)(smem + STAGES * STAGE_BYTES);   // [STAGES] TMA landed (the leader's count both CTAs' bytes)
+  uint8_t* out_smem = smem + STAGES * STAGE_BYTES;
+  uint64_t* full = (uint64_t*)(out_smem + 8 * C::OUT_BYTES);   // [STAGES] TMA landed (the leader's count both CTAs' bytes)
   uint64_t* empty = full + STAGES;                             // [STAGES] MMAs that read the stage have finished
   uint64_t* acc_full = empty + STAGES;                         // accumulator complete
-  uint64_t* acc_empty = acc_full + 1;                          // accumulator in registers (the leader's, by both CTAs' epilogue threads)
+  uint64_t* acc_empty = acc_full + 1;                          // accumulator in registers (the leader's, by both CTAs' epilogue warps)
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + 1);
   volatile uint32_t* abort_word = (volatile uint32_t*)(tmem_slot + 1);
 
@@ -372,12 +423,13 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     tma_prefetch_desc(&tmWs);
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmAs);
+    tma_prefetch_desc(&tmC);
     for (int s = 0; s < STAGES; s++) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 512);
+    mbar_init(acc_empty, 16);      // one arrival a warp: 512 threads' would take longer than the loads they report
     abort_word[0] = abort_word[1] = 0u;
     fence_mbar_init();
   }
@@ -485,10 +537,20 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       for (int c = 0; c < 128; c += 32) tmem_ld32(src + c, v + c);
       tmem_wait_ld();
       tc_fence_before();
-      mbar_arrive_cluster(mapa(smem_u32(acc_empty), 0));
-      const int row = m0 + quarter * 32 + lane, col0 = n0 + half * 128;
-      if (row < p.M && col0 < p.N) pair_store(p, v, row, col0, alpha);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster_relaxed(mapa(smem_u32(acc_empty), 0));
+      const int row0 = m0 + quarter * 32, col0 = n0 + half * 128;
+      if (row0 >= p.M || col0 >= p.N) continue;
+      if (p.epi == KREA_CUDA_EPI_RESID_GATE) {
+        if (row0 + lane < p.M) pair_add(p, v, row0 + lane, col0, alpha);
+      } else {
+        // after a worker's last tile the stages are free: every box of a warp has a place of its own there
+        const bool last = t + workers >= tiles;
+        pair_store(p, tmC, v, row0, col0, alpha, last ? smem + (warp - 4) * 4 * C::OUT_BYTES : out_smem + (warp - 4) * C::OUT_BYTES, last, lane);
+      }
     }
+    if (lane == 0) tma_store_wait_read();      // the last box has left shared memory
+    __syncwarp();
   }
 
   // nobody leaves or frees tensor memory while the peer may still read this CTA's shared memory, signal its barriers or
@@ -519,7 +581,7 @@ static cudaError_t launch_rows_variant(const CUtensorMap& tmA, const CUtensorMap
 }
 
 template <bool MX>
-static cudaError_t launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, Fp4GemmParams p, int sms, bool pdl,
+static cudaError_t launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const CUtensorMap& tmC, Fp4GemmParams p, int sms, bool pdl,
                                        cudaStream_t stream) {
   using namespace fp4g;
   static ConfiguredOnce once;
@@ -534,7 +596,7 @@ static cudaError_t launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap
   if (gmax < 1) gmax = 1;
   const int groups = (int)((mt + gmax - 1) / gmax);
   p.group_m = (mt + groups - 1) / groups;
-  return launch_kernel(gemm_fp4_pair_sm100<MX>, dim3((unsigned)workers * 2), PAIR_THREADS, PairCfg<MX>::SMEM, stream, pdl, 2, true, tmA, tmAs, tmW, tmWs, p);
+  return launch_kernel(gemm_fp4_pair_sm100<MX>, dim3((unsigned)workers * 2), PAIR_THREADS, PairCfg<MX>::SMEM, stream, pdl, 2, true, tmA, tmAs, tmW, tmWs, tmC, p);
 }
 
 Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force) {
@@ -551,10 +613,10 @@ Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force) {
   return plan;
 }
 
-cudaError_t launch_gemm_fp4(const Fp4GemmPlan& plan, const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p,
+cudaError_t launch_gemm_fp4(const Fp4GemmPlan& plan, const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const CUtensorMap& tmC, const Fp4GemmParams& p,
                             int sms, bool pdl, cudaStream_t stream) {
   if (p.M <= 0 || p.N <= 0 || p.K <= 0) return cudaSuccess;
-  if (plan.pair) return p.mx ? launch_pair_variant<true>(tmA, tmAs, tmW, tmWs, p, sms, pdl, stream) : launch_pair_variant<false>(tmA, tmAs, tmW, tmWs, p, sms, pdl, stream);
+  if (plan.pair) return p.mx ? launch_pair_variant<true>(tmA, tmAs, tmW, tmWs, tmC, p, sms, pdl, stream) : launch_pair_variant<false>(tmA, tmAs, tmW, tmWs, tmC, p, sms, pdl, stream);
 #define KREA_ROWS(TN) return p.mx ? launch_rows_variant<true, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, pdl, stream) : launch_rows_variant<false, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, pdl, stream)
   switch (plan.tn) {
     case 16: KREA_ROWS(16);
