@@ -62,8 +62,11 @@ struct Fp4QuantParams {
   int rows, K;
   int64_t ld, ldq;
   int mx;                       // 1: blocks of 32, e8m0 scales; 0: blocks of 16, e4m3 scales
+  uint32_t* status;             // the transposed form reports a wait that ran out here
 };
-cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, bool transposed, bool pdl, cudaStream_t stream);
+cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, bool pdl, cudaStream_t stream);
+// transposed: tm describes src as [K, rows] in boxes of 128 k x 128 rows, no swizzle
+cudaError_t launch_fp4_quantize_cols(const CUtensorMap& tm, const Fp4QuantParams& p, int sms, bool pdl, cudaStream_t stream);
 
 struct Fp4DequantParams {
   const uint8_t* q;
@@ -86,11 +89,13 @@ struct Fp4GemmParams {
   const float* a_ts;            // device scalars, nullptr = 1
   const float* w_ts;
   uint32_t* status;
-  int group_m;                  // set by the launcher: row blocks per group of the tile order
+  int group_m;                  // set by the launcher, CTA pairs: row blocks per group of the tile order
+  int tn, stages;               // set by the launcher, few rows: rows of A a CTA, stages of its ring
 };
 struct Fp4GemmPlan {
   bool pair;                    // 256 x 256 tiles on CTA pairs; else 128 weight columns x tn rows a CTA
-  int tn;                       // rows of A a CTA takes (columns of its tensor-core tile)
+  int tn;                       // rows of A a CTA takes (columns of its tensor-core tile), a multiple of 16
+  int stages;
   int split;                    // CTAs of a cluster that share one tile's K
 };
 // force: 0 = choose by size, 1 = few-rows kernel, 2 = CTA pairs

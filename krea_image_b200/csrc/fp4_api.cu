@@ -46,6 +46,8 @@ static int make_out_map(krea_cuda* h, CUtensorMap* tm, void* base, int rows, int
   return KREA_CUDA_OK;
 }
 
+static int sms(const krea_cuda* h) { return h->sm_count > 0 ? h->sm_count : 148; }
+
 extern "C" {
 
 size_t krea_cuda_fp4_row_bytes(int K) { return K > 0 ? (size_t)fp4_row_bytes(K) : 0; }
@@ -59,7 +61,19 @@ int krea_cuda_fp4_quantize(krea_cuda* h, const krea_cuda_fp4_quantize_args* a) {
   p.src = (const __nv_bfloat16*)a->src; p.q = (uint8_t*)a->q; p.scales = (uint8_t*)a->scales; p.tensor_scale = a->tensor_scale;
   p.rows = a->rows; p.K = a->K; p.ld = a->ld; p.ldq = a->ldq; p.mx = a->format == KREA_CUDA_FP4_MX;
   CUDA_TRY(h, cudaSetDevice(h->device));
-  CUDA_TRY(h, launch_fp4_quantize(p, a->transposed != 0, h->pdl, h->stream));
+  if (a->transposed) {
+    p.status = h->status_dev;
+    cuuint64_t dims[3] = {(cuuint64_t)a->rows, (cuuint64_t)a->K, 1};
+    cuuint64_t strides[2] = {(cuuint64_t)a->ld * 2, (cuuint64_t)a->ld * 2 * (cuuint64_t)a->K};
+    cuuint32_t box[3] = {128, 128, 1}, estr[3] = {1, 1, 1};
+    CUtensorMap tm;
+    CUresult r = h->encode(&tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a->src), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(h, KREA_CUDA_E_CUDA, "fp4_quantize: cuTensorMapEncodeTiled failed with %d", (int)r);
+    CUDA_TRY(h, launch_fp4_quantize_cols(tm, p, sms(h), h->pdl, h->stream));
+  } else {
+    CUDA_TRY(h, launch_fp4_quantize(p, h->pdl, h->stream));
+  }
   h->launches++;
   return KREA_CUDA_OK;
 }
@@ -83,13 +97,8 @@ int krea_cuda_gemm_fp4(krea_cuda* h, const krea_cuda_gemm_fp4_args* a) {
   if (const char* m = check_gemm_fp4(a)) return fail(h, KREA_CUDA_E_ARG, "gemm_fp4: %s", m);
   if (a->M == 0 || a->N == 0) return KREA_CUDA_OK;
   CUDA_TRY(h, cudaSetDevice(h->device));
-  if (h->sm_count == 0) {
-    cudaDeviceProp prop;
-    CUDA_TRY(h, cudaGetDeviceProperties(&prop, h->device));
-    h->sm_count = prop.multiProcessorCount;
-  }
   const bool mx = a->format == KREA_CUDA_FP4_MX;
-  const Fp4GemmPlan plan = plan_gemm_fp4(a->M, a->N, a->K, mx, h->sm_count, h->fp4_tile);
+  const Fp4GemmPlan plan = plan_gemm_fp4(a->M, a->N, a->K, mx, sms(h), h->fp4_tile);
   CUtensorMap tmA, tmAs, tmW, tmWs, tmC;
   memset(&tmC, 0, sizeof(tmC));
   int rc;
@@ -104,7 +113,7 @@ int krea_cuda_gemm_fp4(krea_cuda* h, const krea_cuda_gemm_fp4_args* a) {
   p.vec = uses_vec ? a->vec : nullptr;
   p.a_ts = a->a_tensor_scale; p.w_ts = a->w_tensor_scale;
   p.status = h->status_dev;
-  CUDA_TRY(h, launch_gemm_fp4(plan, tmA, tmAs, tmW, tmWs, tmC, p, h->sm_count, h->pdl, h->stream));
+  CUDA_TRY(h, launch_gemm_fp4(plan, tmA, tmAs, tmW, tmWs, tmC, p, sms(h), h->pdl, h->stream));
   h->launches++;
   return KREA_CUDA_OK;
 }
@@ -119,7 +128,7 @@ int krea_cuda_gated_norm(krea_cuda* h, const krea_cuda_gated_norm_args* a) {
   p.rows = a->rows; p.width = a->width; p.ld_x = a->ld_x; p.ld_y = a->ld_y; p.ld_xo = a->ld_xo; p.ld_h = a->ld_h;
   p.mod_rows = a->mod_rows; p.mod_ld = a->mod_ld; p.x_scale = a->x_scale; p.eps = a->eps; p.y_f32 = a->y_f32 != 0; p.out = a->out;
   CUDA_TRY(h, cudaSetDevice(h->device));
-  CUDA_TRY(h, launch_gated_norm(p, h->sm_count, h->pdl, h->stream));
+  CUDA_TRY(h, launch_gated_norm(p, sms(h), h->pdl, h->stream));
   h->launches++;
   return KREA_CUDA_OK;
 }

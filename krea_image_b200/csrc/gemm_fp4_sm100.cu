@@ -193,33 +193,31 @@ __device__ __forceinline__ void pair_add(const Fp4GemmParams& p, const uint32_t*
 }
 
 // ---------------------------------------------------------------------------------------------- few rows
-template <bool MX, int TN>
-struct RowsCfg {
-  static constexpr int X_BYTES = ROW_TILE_BYTES, Y_BYTES = TN * 128, S_BYTES = scale_chunk(MX);
-  static constexpr int STAGE_BYTES = X_BYTES + Y_BYTES + 2 * S_BYTES;
-  // two CTAs an SM, in shared memory (228 KB, 1 KB of it taken by each CTA) as in tensor memory (512 columns)
-  static constexpr int FIT = (228 * 1024 / 2 - 1024 - 256 - 1024) / STAGE_BYTES, STAGES = FIT < 5 ? FIT : 5;
-  static constexpr int SF_COLS = 2 * 4 * scale_pieces(MX);     // tensor-memory columns of a stage's scales
-  static constexpr int ACC_COLS = TN < 32 ? 32 : TN;
-  static constexpr int TMEM_USED = ACC_COLS + STAGES * SF_COLS;
-  static constexpr int TMEM_COLS = TMEM_USED <= 128 ? 128 : TMEM_USED <= 256 ? 256 : 512;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 256 + 1024;
-};
+// A stage: 128 rows of W, tn rows of A (a multiple of 16), the scales of the row tiles that hold them
+__host__ __device__ constexpr int rows_stage_bytes(bool mx, int tn) { return ROW_TILE_BYTES + tn * 128 + 2 * scale_chunk(mx); }
+__host__ __device__ constexpr int rows_sf_cols(bool mx) { return 2 * 4 * scale_pieces(mx); }      // tensor-memory columns of a stage's scales
+__host__ __device__ constexpr int rows_acc_cols(int tn) { return (tn + 31) & ~31; }
+__host__ __device__ constexpr int rows_tmem_cols(bool mx, int tn, int stages) {
+  const int used = rows_acc_cols(tn) + stages * rows_sf_cols(mx);
+  return used <= 128 ? 128 : used <= 256 ? 256 : 512;
+}
+constexpr int ROWS_MAX_STAGES = 8;
 constexpr int ROWS_THREADS = 192;   // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 }  // namespace fp4g
 
-template <bool MX, int TN>
+template <bool MX>
 __global__ void __launch_bounds__(fp4g::ROWS_THREADS)
 gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs, const __grid_constant__ CUtensorMap tmW,
                     const __grid_constant__ CUtensorMap tmWs, const Fp4GemmParams p) {
   using namespace fp4g;
-  using C = RowsCfg<MX, TN>;
-  constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES, PIECES = scale_pieces(MX);
+  constexpr int PIECES = scale_pieces(MX), S_BYTES = scale_chunk(MX), SF_COLS = rows_sf_cols(MX);
+  const int TN = p.tn, STAGES = p.stages, STAGE_BYTES = rows_stage_bytes(MX, TN), Y_BYTES = TN * 128;
+  const uint32_t TMEM_COLS = (uint32_t)rows_tmem_cols(MX, TN, STAGES);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* full = (uint64_t*)(smem + STAGES * STAGE_BYTES);
-  uint64_t* empty = full + STAGES;
-  uint64_t* acc_full = empty + STAGES;
+  uint64_t* empty = full + ROWS_MAX_STAGES;
+  uint64_t* acc_full = empty + ROWS_MAX_STAGES;
   uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
   volatile uint32_t* abort_word = (volatile uint32_t*)(tmem_slot + 1);
 
@@ -243,46 +241,48 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot, sf_base = tmem_base + C::ACC_COLS;
+  const uint32_t tmem_base = *tmem_slot, sf_base = tmem_base + (uint32_t)rows_acc_cols(TN);
   griddep_wait();
   griddep_launch();
 
   if (warp == 0) {
     if (lane == 0) {
       if (p.status != nullptr && *(volatile uint32_t*)p.status != 0u) abort_word[0] = 0xFFu;      // an earlier kernel gave up: do nothing
-      uint32_t n = 0;
-      for (int kb = kb0; kb < kb1 && *abort_word == 0u; kb++, n++) {
-        const int s = n % STAGES;
-        if (!mbar_wait(&empty[s], ((n / STAGES) & 1) ^ 1, abort_word, SITE_EMPTY)) break;
+      int s = 0, done = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1 && *abort_word == 0u; kb++, done++) {
+        if (!mbar_wait(&empty[s], phase ^ 1u, abort_word, SITE_EMPTY)) break;
         uint8_t* st = smem + s * STAGE_BYTES;
         mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
         tma_load_3d(st, &tmW, &full[s], kb * 128, n0, 0);
-        tma_load_3d(st + C::X_BYTES, &tmA, &full[s], kb * 128, m0, 0);
-        tma_load_3d(st + C::X_BYTES + C::Y_BYTES, &tmWs, &full[s], 0, kb, n0 >> 7);
-        tma_load_3d(st + C::X_BYTES + C::Y_BYTES + C::S_BYTES, &tmAs, &full[s], 0, kb, m0 >> 7);
+        tma_load_3d(st + ROW_TILE_BYTES, &tmA, &full[s], kb * 128, m0, 0);
+        tma_load_3d(st + ROW_TILE_BYTES + Y_BYTES, &tmWs, &full[s], 0, kb, n0 >> 7);
+        tma_load_3d(st + ROW_TILE_BYTES + Y_BYTES + S_BYTES, &tmAs, &full[s], 0, kb, m0 >> 7);
+        if (++s == STAGES) s = 0, phase ^= 1u;
       }
       // nothing may still be in flight into this CTA's shared memory when it exits
       if (*abort_word != 0u) {
-        for (uint32_t i = (n > STAGES ? n - STAGES : 0); i < n; i++) mbar_wait_slow(&full[i % STAGES], (i / STAGES) & 1, abort_word + 1, SITE_FULL);
+        for (int i = done > STAGES ? done - STAGES : 0; i < done; i++) mbar_wait_slow(&full[i % STAGES], (uint32_t)(i / STAGES) & 1u, abort_word + 1, SITE_FULL);
       }
     }
   } else if (warp == 1) {
     const bool leader = elect_one();
-    constexpr uint32_t HI = desc_hi(1024), ID = idesc(MX, 128, TN);
+    constexpr uint32_t HI = desc_hi(1024);
+    const uint32_t ID = idesc(MX, 128, TN);
     const uint32_t smem16 = smem_u32(smem) >> 4;
-    uint32_t n = 0;
-    for (int kb = kb0; kb < kb1; kb++, n++) {
-      const int s = n % STAGES;
-      if (!mbar_wait(&full[s], (n / STAGES) & 1, abort_word, SITE_FULL)) break;
+    int s = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; kb++) {
+      if (!mbar_wait(&full[s], phase, abort_word, SITE_FULL)) break;
       tc_fence_after();
-      const uint32_t x = smem16 + s * (STAGE_BYTES >> 4), y = x + (C::X_BYTES >> 4), sx = y + (C::Y_BYTES >> 4), sy = sx + (C::S_BYTES >> 4);
-      const uint32_t tx = sf_base + s * C::SF_COLS, ty = tx + 4 * PIECES;
+      const uint32_t x = smem16 + s * (STAGE_BYTES >> 4), y = x + (ROW_TILE_BYTES >> 4), sx = y + (Y_BYTES >> 4), sy = sx + (S_BYTES >> 4);
+      const uint32_t tx = sf_base + s * SF_COLS, ty = tx + 4 * PIECES;
       if (leader) {
 #pragma unroll
         for (int j = 0; j < PIECES; j++) {
@@ -297,6 +297,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         umma_commit(&empty[s]);
       }
       __syncwarp();
+      if (++s == STAGES) s = 0, phase ^= 1u;
     }
     if (leader) umma_commit(acc_full);
     __syncwarp();
@@ -316,7 +317,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         tmem_wait_ld();
 #pragma unroll
         for (int e = 0; e < 32; e++)
-          if (TN >= 32 || e < TN) part[(c0 + e) * 128 + quarter * 32 + lane] = __uint_as_float(v[e]);
+          if (c0 + e < TN) part[(c0 + e) * 128 + quarter * 32 + lane] = __uint_as_float(v[e]);
       }
     }
     tc_fence_before();
@@ -336,19 +337,26 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (n0 + c >= p.N) continue;
     float f[8], g[8];
     auto sum = [&](int col, float* o) {
+      float4 a[8][2];
 #pragma unroll
-      for (int e = 0; e < 8; e++) o[e] = 0.f;
-      for (uint32_t q = 0; q < split; q++) {
-        float4 a, b;
+      for (uint32_t q = 0; q < 8; q++) {       // every part is asked for before the first is added
+        if (q >= split) break;
         if (split > 1) {
           const uint32_t at = mapa(smem_u32(part + r * 128 + col), q);
-          a = ld_cluster_f32x4(at);
-          b = ld_cluster_f32x4(at + 16);
+          a[q][0] = ld_cluster_f32x4(at);
+          a[q][1] = ld_cluster_f32x4(at + 16);
         } else {
-          a = *(const float4*)(part + r * 128 + col);
-          b = *(const float4*)(part + r * 128 + col + 4);
+          a[q][0] = *(const float4*)(part + r * 128 + col);
+          a[q][1] = *(const float4*)(part + r * 128 + col + 4);
         }
-        o[0] += a.x; o[1] += a.y; o[2] += a.z; o[3] += a.w; o[4] += b.x; o[5] += b.y; o[6] += b.z; o[7] += b.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e] = 0.f;
+#pragma unroll
+      for (uint32_t q = 0; q < 8; q++) {
+        if (q >= split) break;
+        o[0] += a[q][0].x; o[1] += a[q][0].y; o[2] += a[q][0].z; o[3] += a[q][0].w;
+        o[4] += a[q][1].x; o[5] += a[q][1].y; o[6] += a[q][1].z; o[7] += a[q][1].w;
       }
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] *= alpha;
@@ -368,7 +376,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   if (split > 1) cluster_sync_all();       // nobody leaves while the others still read its part
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, C::TMEM_COLS);
+    tmem_dealloc(tmem_base, TMEM_COLS);
   }
   if (threadIdx.x == 0 && p.status != nullptr) {
     const uint32_t a = *abort_word;
@@ -569,15 +577,16 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
 }
 
-template <bool MX, int TN>
+template <bool MX>
 static cudaError_t launch_rows_variant(const CUtensorMap& tmA, const CUtensorMap& tmAs, const CUtensorMap& tmW, const CUtensorMap& tmWs, const Fp4GemmParams& p, int split, bool pdl,
                                        cudaStream_t stream) {
   using namespace fp4g;
   static ConfiguredOnce once;
-  cudaError_t e = once.set(gemm_fp4_rows_sm100<MX, TN>, RowsCfg<MX, TN>::SMEM);
+  cudaError_t e = once.set(gemm_fp4_rows_sm100<MX>, 227 * 1024);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)((p.N + 127) / 128), (unsigned)((p.M + TN - 1) / TN), (unsigned)split);
-  return launch_kernel(gemm_fp4_rows_sm100<MX, TN>, grid, ROWS_THREADS, RowsCfg<MX, TN>::SMEM, stream, pdl, split, false, tmA, tmAs, tmW, tmWs, p);
+  const dim3 grid((unsigned)((p.N + 127) / 128), (unsigned)((p.M + p.tn - 1) / p.tn), (unsigned)split);
+  const size_t smem = (size_t)p.stages * rows_stage_bytes(MX, p.tn) + 256 + 1024;
+  return launch_kernel(gemm_fp4_rows_sm100<MX>, grid, ROWS_THREADS, smem, stream, pdl, split, false, tmA, tmAs, tmW, tmWs, p);
 }
 
 template <bool MX>
@@ -600,16 +609,35 @@ static cudaError_t launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap
 }
 
 Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force) {
-  (void)mx;
   Fp4GemmPlan plan{};
   plan.split = 1;
-  plan.pair = force == 2 || (force == 0 && M > 256);
+  plan.pair = force == 2 || (force == 0 && M > 128);
   if (plan.pair) return plan;
-  plan.tn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + plan.tn - 1) / plan.tn);
+  // rows of A a CTA: all of them up to 128, in whole sixteens; above, tiles of 128 (a tile starts where its scales do)
+  const int shares = (M + 127) / 128;
+  plan.tn = M < 128 ? (M + 15) & ~15 : 128;
+  const int64_t tiles = (int64_t)((N + 127) / 128) * shares;
   const int kblocks = (K + fp4g::KB - 1) / fp4g::KB;
-  // enough CTAs to fill the SMs, at least two stages of K each
-  while (plan.split < 8 && tiles * plan.split * 2 <= 2 * sms && kblocks >= plan.split * 4) plan.split *= 2;
+  // How K is shared.  One CTA an SM with a deep ring is best as long as clusters find room side by side (up to five SMs in six;
+  // 48 clusters of three on 148 SMs did not, and ran in two rounds); with few rows and not even three quarters of the SMs
+  // busy that way, two CTAs an SM with short rings.  us at K = 6144 (NV): 1 x 6144 deep 2 x 48 CTAs 8.2, short 4 x 48 6.8;
+  // 1 x 15360 deep 120 11.3, short 240 11.9; 128 x 6144 deep 2 x 48 11.8, short 3 x 48 14.4; 77 x 15360 deep 120 14.2, short
+  // 240 16.6.
+  const auto most = [&](int64_t ctas, int top) {
+    int c = 1;
+    while (c < top && tiles * (c + 1) <= ctas && kblocks > c) c++;
+    return c;
+  };
+  plan.split = most(sms * 5 / 6, 8);
+  int ctas = tiles * plan.split > sms ? 2 : 1;      // a SM
+  if (ctas == 1 && plan.tn <= 32 && tiles * plan.split * 4 < 3 * (int64_t)sms) {
+    plan.split = most(sms * 5 / 3, 5);
+    ctas = 2;
+  }
+  const int room = 228 * 1024 / ctas - 1024 - 256 - 1024;
+  plan.stages = room / fp4g::rows_stage_bytes(mx != 0, plan.tn);
+  if (plan.stages > fp4g::ROWS_MAX_STAGES) plan.stages = fp4g::ROWS_MAX_STAGES;
+  while (fp4g::rows_tmem_cols(mx != 0, plan.tn, plan.stages) > 512 / ctas) plan.stages--;
   return plan;
 }
 
@@ -617,14 +645,10 @@ cudaError_t launch_gemm_fp4(const Fp4GemmPlan& plan, const CUtensorMap& tmA, con
                             int sms, bool pdl, cudaStream_t stream) {
   if (p.M <= 0 || p.N <= 0 || p.K <= 0) return cudaSuccess;
   if (plan.pair) return p.mx ? launch_pair_variant<true>(tmA, tmAs, tmW, tmWs, tmC, p, sms, pdl, stream) : launch_pair_variant<false>(tmA, tmAs, tmW, tmWs, tmC, p, sms, pdl, stream);
-#define KREA_ROWS(TN) return p.mx ? launch_rows_variant<true, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, pdl, stream) : launch_rows_variant<false, TN>(tmA, tmAs, tmW, tmWs, p, plan.split, pdl, stream)
-  switch (plan.tn) {
-    case 16: KREA_ROWS(16);
-    case 32: KREA_ROWS(32);
-    case 64: KREA_ROWS(64);
-    default: KREA_ROWS(128);
-  }
-#undef KREA_ROWS
+  Fp4GemmParams q = p;
+  q.tn = plan.tn;
+  q.stages = plan.stages;
+  return p.mx ? launch_rows_variant<true>(tmA, tmAs, tmW, tmWs, q, plan.split, pdl, stream) : launch_rows_variant<false>(tmA, tmAs, tmW, tmWs, q, plan.split, pdl, stream);
 }
 
 }  // namespace krea
