@@ -17,6 +17,9 @@ inline int64_t fp4_row_bytes(int64_t K) { return (K + 31) / 32 * 16; }
 inline int64_t fp4_scale_tile_bytes(int format) { return format == KREA_CUDA_FP4_MX ? 1024 : 2048; }
 inline int64_t fp4_scale_bytes(int format, int64_t rows, int64_t K) { return (rows + 127) / 128 * ((K + 255) / 256) * fp4_scale_tile_bytes(format); }
 
+// sizes beyond this are refused: rounding them up to whole tiles stays within 32 bits
+constexpr int FP4_MAX_SIZE = 1 << 30;
+
 inline bool off16(const void* p) { return ((uintptr_t)p & 15u) != 0; }
 
 // whether the n bytes at a and the m bytes at b have a byte in common
@@ -29,6 +32,7 @@ inline int64_t span(int64_t rows, int64_t width, int64_t ld) { return rows > 0 ?
 
 inline const char* check_fp4_quantize(const krea_cuda_fp4_quantize_args* a) {
   if (a->rows < 0 || a->K < 0) return "negative size";
+  if (a->rows > FP4_MAX_SIZE || a->K > FP4_MAX_SIZE) return "rows and K must be 2^30 at most";
   if (!fp4_format_ok(a->format)) return "format must be KREA_CUDA_FP4_MX or KREA_CUDA_FP4_NV";
   if (a->rows == 0 || a->K == 0) return nullptr;
   if (!a->src || !a->q || !a->scales) return "null tensor";
@@ -45,6 +49,7 @@ inline const char* check_fp4_quantize(const krea_cuda_fp4_quantize_args* a) {
 
 inline const char* check_fp4_dequantize(const krea_cuda_fp4_dequantize_args* a) {
   if (a->rows < 0 || a->K < 0) return "negative size";
+  if (a->rows > FP4_MAX_SIZE || a->K > FP4_MAX_SIZE) return "rows and K must be 2^30 at most";
   if (!fp4_format_ok(a->format)) return "format must be KREA_CUDA_FP4_MX or KREA_CUDA_FP4_NV";
   if (a->rows == 0 || a->K == 0) return nullptr;
   if (!a->q || !a->scales || !a->out) return "null tensor";
@@ -67,6 +72,7 @@ inline bool epilogue_f32(int e) { return e == KREA_CUDA_EPI_RESID_GATE || e == K
 
 inline const char* check_gemm_fp4(const krea_cuda_gemm_fp4_args* a) {
   if (a->M < 0 || a->N < 0 || a->K < 0) return "negative size";
+  if (a->M > FP4_MAX_SIZE || a->N > FP4_MAX_SIZE || a->K > FP4_MAX_SIZE) return "M, N and K must be 2^30 at most";
   if (!fp4_format_ok(a->format)) return "format must be KREA_CUDA_FP4_MX or KREA_CUDA_FP4_NV";
   if (a->M == 0 || a->N == 0) return nullptr;
   if (a->K == 0) return "K must be positive";
@@ -93,6 +99,7 @@ constexpr int GATED_NORM_MAX_WIDTH = 32768;
 
 inline const char* check_gated_norm(const krea_cuda_gated_norm_args* a) {
   if (a->rows < 0 || a->width < 0) return "negative size";
+  if (a->rows > FP4_MAX_SIZE) return "rows must be 2^30 at most";
   if (a->out < KREA_CUDA_OUT_BF16 || a->out > KREA_CUDA_OUT_FP4_NV) return "out must be one of KREA_CUDA_OUT_*";
   if (a->rows == 0 || a->width == 0) return nullptr;
   if (!a->x || !(a->x_out || a->h)) return "null tensor";

@@ -58,7 +58,10 @@ class _Call:
         self.pack = struct.Struct("@" + "".join(self._CODES[t] for _, t in cls._fields_)).pack_into
 
     def __call__(self, h, *values):
-        self.pack(self.buf, 0, *values)
+        try:
+            self.pack(self.buf, 0, *values)
+        except struct.error as e:          # a size beyond 32 bits, or no whole number
+            raise KreaCudaError(B.E_ARG, f"argument out of range: {e}") from None
         return self.fn(h, self.ref)
 
 

@@ -80,7 +80,7 @@ def _try(fn, cls, good, changes):
 def test_quantize_refusals(checks):
     good = dict(src=P[0], q=P[1], scales=P[2], tensor_scale=P[3], rows=5, K=70, ld=72, ldq=48, format=B.FP4_NV, transposed=0)
     _try(checks.fp4_quantize, B.Fp4QuantizeArgs, good, [
-        dict(rows=-1), dict(K=-1), dict(format=2), dict(format=-1), dict(src=None), dict(q=None), dict(scales=None),
+        dict(rows=-1), dict(K=-1), dict(rows=(1 << 30) + 1), dict(K=(1 << 30) + 1, ld=0x7FFFFFF8, ldq=0x7FFFFFF0), dict(format=2), dict(format=-1), dict(src=None), dict(q=None), dict(scales=None),
         dict(src=P[0] + 8), dict(q=P[1] + 4), dict(scales=P[2] + 2), dict(tensor_scale=P[3] + 2), dict(format=B.FP4_MX), dict(ld=68), dict(ld=76), dict(ldq=32),
         dict(ldq=50), dict(transposed=1, rows=80), dict(q=P[0]), dict(scales=P[0] + 16), dict(scales=P[1]), dict(scales=P[1] + 4 * 48 + 32)])
     for ch in (dict(rows=0, src=None), dict(K=0, q=None), dict(tensor_scale=None), dict(transposed=1, ld=8), dict(format=B.FP4_MX, tensor_scale=None)):
@@ -98,7 +98,7 @@ def test_gemm_refusals(checks):
     good = dict(A=P[0], a_scales=P[1], W=P[2], w_scales=P[3], C=P[4], M=3, N=64, K=70, lda=48, ldw=64, ldc=64, format=B.FP4_NV, epilogue=B.EPI_BF16, vec=P[5],
                 a_tensor_scale=P[6], w_tensor_scale=P[7])
     _try(checks.gemm_fp4, B.GemmFp4Args, good, [
-        dict(M=-1), dict(N=-8), dict(K=-1), dict(K=0), dict(format=3), dict(A=None), dict(a_scales=None), dict(W=None), dict(w_scales=None), dict(C=None),
+        dict(M=-1), dict(N=-8), dict(K=-1), dict(K=0), dict(M=(1 << 30) + 1), dict(N=(1 << 30) + 8, ldc=(1 << 30) + 8), dict(K=0x7FFFFFFF, lda=0x7FFFFFF0, ldw=0x7FFFFFF0), dict(format=3), dict(A=None), dict(a_scales=None), dict(W=None), dict(w_scales=None), dict(C=None),
         dict(A=P[0] + 8), dict(a_scales=P[1] + 8), dict(W=P[2] + 8), dict(w_scales=P[3] + 8), dict(C=P[4] + 8), dict(a_tensor_scale=P[6] + 2), dict(w_tensor_scale=P[7] + 1),
         dict(format=B.FP4_MX), dict(lda=32), dict(lda=56), dict(ldw=32), dict(ldw=72), dict(N=60), dict(ldc=66), dict(ldc=56), dict(epilogue=B.EPI_SWIGLU, N=32),
         dict(epilogue=B.EPI_BIAS_BF16, vec=None), dict(epilogue=B.EPI_BIAS_F32, vec=P[5] + 4), dict(epilogue=B.EPI_RESID_GATE, vec=P[5] + 8), dict(C=P[0]), dict(C=P[2] + 64),
@@ -111,7 +111,7 @@ def test_gated_norm_refusals(checks):
     good = dict(x=P[0], y=P[1], x_out=P[2], h=P[3], h_scales=P[4], h_tensor_scale=P[5], post=P[6], gate=P[7], mul=P[8], add=P[9], rows=5, width=40, ld_x=44, ld_y=40, ld_xo=40, ld_h=32,
                 mod_rows=2, mod_ld=40, x_scale=1.0, eps=1e-6, y_f32=0, out=B.OUT_FP4_NV)
     _try(checks.gated_norm, B.GatedNormArgs, good, [
-        dict(rows=-1), dict(width=-8), dict(out=4), dict(out=-1), dict(x=None), dict(x_out=None, h=None), dict(width=36), dict(width=32776, ld_x=32776, ld_y=32776, ld_xo=32776, ld_h=16400),
+        dict(rows=-1), dict(rows=(1 << 30) + 1), dict(width=-8), dict(out=4), dict(out=-1), dict(x=None), dict(x_out=None, h=None), dict(width=36), dict(width=32776, ld_x=32776, ld_y=32776, ld_xo=32776, ld_h=16400),
         dict(ld_x=36), dict(ld_x=42), dict(ld_y=44), dict(ld_y=32), dict(ld_xo=36), dict(ld_xo=41), dict(y=None), dict(y=None, post=None), dict(mul=None), dict(ld_h=16), dict(ld_h=40),
         dict(h_scales=None), dict(out=B.OUT_FP4_MX), dict(out=B.OUT_BF16, ld_h=40), dict(h_tensor_scale=P[5] + 2), dict(x=P[0] + 4), dict(y=P[1] + 2), dict(x_out=P[2] + 8), dict(h=P[3] + 8),
         dict(post=P[6] + 4), dict(gate=P[7] + 4), dict(mul=P[8] + 4), dict(add=P[9] + 4), dict(h_scales=P[4] + 4), dict(mod_rows=-1), dict(mod_ld=42), dict(mod_ld=-4),
