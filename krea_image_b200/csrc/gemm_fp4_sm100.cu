@@ -205,6 +205,18 @@ constexpr int ROWS_MAX_STAGES = 8;
 constexpr int ROWS_THREADS = 192;   // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 }  // namespace fp4g
 
+// up to 32 rows of one column, 512 bytes apart, in this CTA's shared memory or another's
+template <bool CLUSTER>
+__device__ __forceinline__ void put_rows(uint32_t at, const uint32_t* v, int n) {
+#pragma unroll
+  for (int e = 0; e < 32; e++) {
+    if (e < n) {
+      if constexpr (CLUSTER) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at + e * 512), "r"(v[e]) : "memory");
+      else asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + e * 512), "r"(v[e]) : "memory");
+    }
+  }
+}
+
 template <bool MX>
 __global__ void __launch_bounds__(fp4g::ROWS_THREADS)
 gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs, const __grid_constant__ CUtensorMap tmW,
@@ -302,61 +314,56 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (leader) umma_commit(acc_full);
     __syncwarp();
   }
-  // tensor memory -> shared memory as [row of A][128 columns of C] f32, over the stages, which nothing uses any more
+  // Each CTA of the cluster finishes an equal share of the tile's rows.  The parts of a row go straight from tensor memory
+  // to the shared memory of the CTA that finishes it, as [CTA they come from][row][128 columns of C] f32, over its
+  // stages: stores have no latency to wait for, and after them nobody touches another CTA's memory.
   float* part = (float*)smem;
+  const int rows = min(TN, p.M - m0), share = (rows + (int)split - 1) / (int)split;
+  bool done = true;
   if (warp >= 2) {
-    const int quarter = warp & 3;
-    const bool ok = mbar_wait(acc_full, 0, abort_word, SITE_ACC_FULL);
+    done = mbar_wait(acc_full, 0, abort_word, SITE_ACC_FULL);
     tc_fence_after();
-    if (ok) {
+  }
+  __syncwarp();
+  if (split > 1) cluster_sync_all();         // no CTA's stages are in use any more
+  if (warp >= 2 && done) {
+    const int quarter = warp & 3;
+    for (uint32_t q = 0; q < split; q++) {   // CTA q's rows
+      const int first = (int)q * share, n = min(rows - first, share);
+      const uint32_t here = smem_u32(part + (int)rank * share * 128 + quarter * 32 + lane), to = split > 1 ? mapa(here, q) : here;
 #pragma unroll 1
-      for (int c0 = 0; c0 < TN; c0 += 32) {
-        if (m0 + c0 >= p.M) break;
+      for (int c0 = 0; c0 < n; c0 += 32) {
         uint32_t v[32];
-        tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + c0, v);
+        tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(first + c0), v);
         tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 32; e++)
-          if (c0 + e < TN) part[(c0 + e) * 128 + quarter * 32 + lane] = __uint_as_float(v[e]);
+        const uint32_t at = to + (uint32_t)c0 * 512u;
+        if (split > 1) put_rows<true>(at, v, n - c0);
+        else put_rows<false>(at, v, n - c0);
       }
     }
     tc_fence_before();
   }
   __syncwarp();
-  __syncthreads();
   if (split > 1) cluster_sync_all();
+  else __syncthreads();
 
-  // every CTA of the cluster finishes its share of the tile: 8 columns of one row at a time, parts added in rank order
+  // parts added in rank order, 8 columns of a row at a time
   const bool swiglu = p.epi == KREA_CUDA_EPI_SWIGLU;
-  const int rows = min(TN, p.M - m0), units_row = swiglu ? 8 : 16;
+  const int units_row = swiglu ? 8 : 16, r0 = (int)rank * share, mine = min(rows - r0, share);
   const float alpha = tensor_scale(p);
   const bool live = *abort_word == 0u;
-  for (int u = rank * ROWS_THREADS + threadIdx.x; live && u < rows * units_row; u += split * ROWS_THREADS) {
+  for (int u = threadIdx.x; live && u < mine * units_row; u += ROWS_THREADS) {
     const int r = u / units_row, uc = u % units_row;
     const int c = swiglu ? (uc >> 2) * 64 + (uc & 3) * 8 : uc * 8;       // first of the tile's columns (SwiGLU: of the gate's)
     if (n0 + c >= p.N) continue;
     float f[8], g[8];
-    auto sum = [&](int col, float* o) {
-      float4 a[8][2];
-#pragma unroll
-      for (uint32_t q = 0; q < 8; q++) {       // every part is asked for before the first is added
-        if (q >= split) break;
-        if (split > 1) {
-          const uint32_t at = mapa(smem_u32(part + r * 128 + col), q);
-          a[q][0] = ld_cluster_f32x4(at);
-          a[q][1] = ld_cluster_f32x4(at + 16);
-        } else {
-          a[q][0] = *(const float4*)(part + r * 128 + col);
-          a[q][1] = *(const float4*)(part + r * 128 + col + 4);
-        }
-      }
+    const auto sum = [&](int col, float* o) {
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] = 0.f;
-#pragma unroll
-      for (uint32_t q = 0; q < 8; q++) {
-        if (q >= split) break;
-        o[0] += a[q][0].x; o[1] += a[q][0].y; o[2] += a[q][0].z; o[3] += a[q][0].w;
-        o[4] += a[q][1].x; o[5] += a[q][1].y; o[6] += a[q][1].z; o[7] += a[q][1].w;
+      for (uint32_t q = 0; q < split; q++) {
+        const float4* at = (const float4*)(part + ((int)q * share + r) * 128 + col);
+        const float4 x = at[0], y = at[1];
+        o[0] += x.x; o[1] += x.y; o[2] += x.z; o[3] += x.w; o[4] += y.x; o[5] += y.y; o[6] += y.z; o[7] += y.w;
       }
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] *= alpha;
@@ -369,11 +376,10 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       for (int e = 0; e < 8; e++) f[e] = f[e] * sigmoid_approx(f[e]) * g[e];
       col = ((n0 + c) >> 6) * 32 + (uc & 3) * 8;
     }
-    finish8(p, f, m0 + r, col);
+    finish8(p, f, m0 + r0 + r, col);
   }
   __syncwarp();
   __syncthreads();
-  if (split > 1) cluster_sync_all();       // nobody leaves while the others still read its part
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, TMEM_COLS);

@@ -57,11 +57,5 @@ __device__ __forceinline__ void umma_ss2(uint32_t d_tmem, uint64_t adesc, uint64
 __device__ __forceinline__ void umma_commit2(uint32_t bar_cluster_addr) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
-// f32 from the shared memory of another CTA of the cluster
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
-  return v;
-}
 
 }  // namespace krea
