@@ -20,9 +20,12 @@ namespace krea {
 
 constexpr int FQ_THREADS = 256;
 
-// 16 values from `src` (16-byte aligned), zero from index `left` on
-__device__ __forceinline__ void load16(const __nv_bfloat16* src, int left, uint32_t* w) {
-  if (left >= 16) {
+// 16 values from `src` (16-byte aligned; `wide`: 32), zero from index `left` on
+__device__ __forceinline__ void load16(const __nv_bfloat16* src, int left, bool wide, uint32_t* w) {
+  if (left >= 16 && wide) {       // one access a lane and not two, 32 bytes apart, that cost L1 twice the passes
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(src));
+  } else if (left >= 16) {
     const uint4 a = __ldg((const uint4*)src), b = __ldg((const uint4*)src + 1);
     w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
     w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
@@ -52,6 +55,7 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_quantize_rows_kernel(const Fp4
     __syncthreads();
   }
   const int64_t step = (int64_t)gridDim.x * (FQ_THREADS / 32);
+  const bool wide = (((uintptr_t)p.src | (uintptr_t)(p.ld * 2)) & 31u) == 0;
   for (int64_t it = (int64_t)blockIdx.x * (FQ_THREADS / 32) + (threadIdx.x >> 5); it < items; it += step) {
     const int g = (int)(it % (groups / 2)) * 2;
     const int64_t tr = it / (groups / 2);
@@ -62,7 +66,7 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_quantize_rows_kernel(const Fp4
 #pragma unroll
     for (int i = 0; i < 2; i++) {                // both loads are under way before the first is used
       const int k0 = (g + i) * GROUP + in_row * 16;
-      load16(src + k0, row < p.rows ? p.K - k0 : 0, w[i]);
+      load16(src + k0, row < p.rows ? p.K - k0 : 0, wide, w[i]);
     }
 #pragma unroll
     for (int i = 0; i < 2; i++) {
@@ -208,6 +212,7 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_dequantize_kernel(const Fp4Deq
   const int64_t chunks = (p.K + 255) / 256;
   const int per_row = (p.K + 15) / 16;                 // 16 values a thread
   const int64_t items = (int64_t)p.rows * per_row, step = (int64_t)gridDim.x * FQ_THREADS;
+  const bool wide = (((uintptr_t)p.out | (uintptr_t)(p.ldo * 2)) & 31u) == 0;
   griddep_wait();
   const float ts = MX || !p.tensor_scale ? 1.f : __ldg(p.tensor_scale);
   for (int64_t it = (int64_t)blockIdx.x * FQ_THREADS + threadIdx.x; it < items; it += step) {
@@ -226,7 +231,9 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_dequantize_kernel(const Fp4Deq
       out[i] = pack_bf16x2(f.x * s * ts, f.y * s * ts);
     }
     __nv_bfloat16* dst = p.out + (int64_t)row * p.ldo + k0;
-    if (p.K - k0 >= 16) {
+    if (p.K - k0 >= 16 && wide) {
+      st_global_32B(dst, out);
+    } else if (p.K - k0 >= 16) {
       *(uint4*)dst = make_uint4(out[0], out[1], out[2], out[3]);
       *((uint4*)dst + 1) = make_uint4(out[4], out[5], out[6], out[7]);
     } else {

@@ -406,6 +406,9 @@ struct PairCfg {
   static_assert(8 * 4 * OUT_BYTES <= STAGES * STAGE_BYTES, "the last tile's boxes lie over the stages");
   static_assert(ACC_COLS + STAGES * SF_COLS <= TMEM_COLS && SMEM <= 227 * 1024, "tile does not fit");
 };
+// ns between the output of one epilogue warp and the next, for each stage of K (340 ns of products): seven such steps, twice as
+// long at worst, end before the next tile does
+constexpr int PACE_NS = 22;
 constexpr int PAIR_THREADS = 384;   // warp 0 TMA, warp 1 MMA, warps 4-11 epilogue (two for each quarter of the tensor-memory lanes)
 }  // namespace fp4g
 
@@ -560,6 +563,9 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       } else {
         // after a worker's last tile the stages are free: every box of a warp has a place of its own there
         const bool last = t + workers >= tiles;
+        // All pairs end their tiles at about the same time, and 64 KB from every SM at once hold up the loads of the next ones:
+        // the warps take turns over the next tile's products (4608 x 15360 x 6144: 183 -> 177 us NV, 176 -> 170 us MX)
+        if (!last) __nanosleep((uint32_t)((warp - 4) * kblocks * PACE_NS));
         pair_store(p, tmC, v, row0, col0, alpha, last ? smem + (warp - 4) * 4 * C::OUT_BYTES : out_smem + (warp - 4) * C::OUT_BYTES, last, lane);
       }
     }
@@ -624,20 +630,21 @@ Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force) {
   plan.tn = M < 128 ? (M + 15) & ~15 : 128;
   const int64_t tiles = (int64_t)((N + 127) / 128) * shares;
   const int kblocks = (K + fp4g::KB - 1) / fp4g::KB;
-  // How K is shared.  One CTA an SM with a deep ring is best as long as clusters find room side by side (up to five SMs in six;
-  // 48 clusters of three on 148 SMs did not, and ran in two rounds); with few rows and not even three quarters of the SMs
-  // busy that way, two CTAs an SM with short rings.  us at K = 6144 (NV): 1 x 6144 deep 2 x 48 CTAs 8.2, short 4 x 48 6.8;
-  // 1 x 15360 deep 120 11.3, short 240 11.9; 128 x 6144 deep 2 x 48 11.8, short 3 x 48 14.4; 77 x 15360 deep 120 14.2, short
-  // 240 16.6.
-  const auto most = [&](int64_t ctas, int top) {
+  // How K is shared: clusters of up to four CTAs (eight where a few tiles are all there is).  One CTA an SM with a deep ring
+  // moves the most while clusters find room side by side: pairs on all SMs, larger ones on five in six (48 clusters of three
+  // on 148 SMs ran in two rounds).  Where that leaves a quarter of the SMs idle and a CTA has at most 64 rows to finish, two
+  // CTAs an SM with short rings.  us, MX, K = 6144: 1 x 6144 deep 2 x 48 CTAs 7.7, short 4 x 48 6.1; 48 x 6144 8.5, 8.0;
+  // 77 x 6144 (K 16384) 16.1, 16.9; 128 x 6144 10.7, 12.3; 1 x 15360 deep 120 11.3, short 240 11.9; 64 x 8192 (K 2048) deep 1 x 64 7.0, 2 x 64 6.5.
+  const int top = tiles * 16 <= sms ? 8 : 4;
+  const auto most = [&](auto room) {
     int c = 1;
-    while (c < top && tiles * (c + 1) <= ctas && kblocks > c) c++;
+    while (c < top && tiles * (c + 1) <= room(c + 1) && kblocks > c) c++;
     return c;
   };
-  plan.split = most(sms * 5 / 6, 8);
+  plan.split = most([&](int c) { return c == 2 ? sms : sms * 5 / 6; });
   int ctas = tiles * plan.split > sms ? 2 : 1;      // a SM
-  if (ctas == 1 && plan.tn <= 32 && tiles * plan.split * 4 < 3 * (int64_t)sms) {
-    plan.split = most(sms * 5 / 3, 5);
+  if (ctas == 1 && plan.tn <= 64 && tiles * plan.split * 4 < 3 * (int64_t)sms) {
+    plan.split = most([&](int) { return sms * 4 / 3; });
     ctas = 2;
   }
   const int room = 228 * 1024 / ctas - 1024 - 256 - 1024;
