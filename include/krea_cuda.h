@@ -373,8 +373,8 @@ KREA_CUDA_API int krea_cuda_dit_block(krea_cuda* h, const krea_cuda_dit_block_ar
  * bytes, values past K zero.  ldq, lda and ldw are in BYTES, multiples of 16.
  * Scales: krea_cuda_fp4_scale_bytes bytes, tiles of 128 rows x 256 values, [row / 128][k / 256][4 blocks][row % 32]
  * [row / 32 % 4][block % 4], zero past K and past the last row.  The product reads the scales past K: they must not be NaN.
- * Every size may be 2^30 at most.  None of these calls allocates, keeps or shares device memory: they can be captured into
- * CUDA graphs and run beside one another.  Outputs may not overlap inputs (x_out of krea_cuda_gated_norm may be x). */
+ * Rows and columns may be 2^30 at most, K 2^26.  None of these calls allocates, keeps or shares device memory: they can be captured into
+ * CUDA graphs and run beside one another.  Outputs may not overlap inputs (x_out of krea_cuda_gated_norm may be x, C of _RESID_GATE is read and written). */
 #define KREA_CUDA_FP4_MX 0
 #define KREA_CUDA_FP4_NV 1
 KREA_CUDA_API size_t krea_cuda_fp4_row_bytes(int K);

@@ -17,8 +17,9 @@ inline int64_t fp4_row_bytes(int64_t K) { return (K + 31) / 32 * 16; }
 inline int64_t fp4_scale_tile_bytes(int format) { return format == KREA_CUDA_FP4_MX ? 1024 : 2048; }
 inline int64_t fp4_scale_bytes(int format, int64_t rows, int64_t K) { return (rows + 127) / 128 * ((K + 255) / 256) * fp4_scale_tile_bytes(format); }
 
-// sizes beyond this are refused: rounding them up to whole tiles stays within 32 bits
-constexpr int FP4_MAX_SIZE = 1 << 30;
+// sizes beyond these are refused: rounding them up to whole tiles stays within 32 bits, and the product's longest wait
+// (for a whole tile's K) far below the limit of two seconds on every wait
+constexpr int FP4_MAX_ROWS = 1 << 30, FP4_MAX_K = 1 << 26;
 
 inline bool off16(const void* p) { return ((uintptr_t)p & 15u) != 0; }
 
@@ -32,7 +33,7 @@ inline int64_t span(int64_t rows, int64_t width, int64_t ld) { return rows > 0 ?
 
 inline const char* check_fp4_quantize(const krea_cuda_fp4_quantize_args* a) {
   if (a->rows < 0 || a->K < 0) return "negative size";
-  if (a->rows > FP4_MAX_SIZE || a->K > FP4_MAX_SIZE) return "rows and K must be 2^30 at most";
+  if (a->rows > FP4_MAX_ROWS || a->K > FP4_MAX_K) return "rows must be 2^30 at most, K 2^26";
   if (!fp4_format_ok(a->format)) return "format must be KREA_CUDA_FP4_MX or KREA_CUDA_FP4_NV";
   if (a->rows == 0 || a->K == 0) return nullptr;
   if (!a->src || !a->q || !a->scales) return "null tensor";
@@ -44,12 +45,13 @@ inline const char* check_fp4_quantize(const krea_cuda_fp4_quantize_args* a) {
   const int64_t qb = span(a->rows, fp4_row_bytes(a->K), a->ldq), sb = fp4_scale_bytes(a->format, a->rows, a->K);
   const int64_t src = a->transposed ? span(a->K, 2 * (int64_t)a->rows, 2 * (int64_t)a->ld) : span(a->rows, 2 * (int64_t)a->K, 2 * (int64_t)a->ld);
   if (overlap(a->q, qb, a->scales, sb) || overlap(a->q, qb, a->src, src) || overlap(a->scales, sb, a->src, src)) return "tensors overlap";
+  if (overlap(a->q, qb, a->tensor_scale, 4) || overlap(a->scales, sb, a->tensor_scale, 4)) return "tensors overlap";
   return nullptr;
 }
 
 inline const char* check_fp4_dequantize(const krea_cuda_fp4_dequantize_args* a) {
   if (a->rows < 0 || a->K < 0) return "negative size";
-  if (a->rows > FP4_MAX_SIZE || a->K > FP4_MAX_SIZE) return "rows and K must be 2^30 at most";
+  if (a->rows > FP4_MAX_ROWS || a->K > FP4_MAX_K) return "rows must be 2^30 at most, K 2^26";
   if (!fp4_format_ok(a->format)) return "format must be KREA_CUDA_FP4_MX or KREA_CUDA_FP4_NV";
   if (a->rows == 0 || a->K == 0) return nullptr;
   if (!a->q || !a->scales || !a->out) return "null tensor";
@@ -60,7 +62,7 @@ inline const char* check_fp4_dequantize(const krea_cuda_fp4_dequantize_args* a) 
   if (a->ldo % 8 || a->ldo < a->K) return "ldo must be a multiple of 8 and cover a row";
   const int64_t qb = span(a->rows, fp4_row_bytes(a->K), a->ldq), sb = fp4_scale_bytes(a->format, a->rows, a->K);
   const int64_t ob = span(a->rows, 2 * (int64_t)a->K, 2 * (int64_t)a->ldo);
-  if (overlap(a->out, ob, a->q, qb) || overlap(a->out, ob, a->scales, sb)) return "tensors overlap";
+  if (overlap(a->out, ob, a->q, qb) || overlap(a->out, ob, a->scales, sb) || overlap(a->out, ob, a->tensor_scale, 4)) return "tensors overlap";
   return nullptr;
 }
 
@@ -72,7 +74,7 @@ inline bool epilogue_f32(int e) { return e == KREA_CUDA_EPI_RESID_GATE || e == K
 
 inline const char* check_gemm_fp4(const krea_cuda_gemm_fp4_args* a) {
   if (a->M < 0 || a->N < 0 || a->K < 0) return "negative size";
-  if (a->M > FP4_MAX_SIZE || a->N > FP4_MAX_SIZE || a->K > FP4_MAX_SIZE) return "M, N and K must be 2^30 at most";
+  if (a->M > FP4_MAX_ROWS || a->N > FP4_MAX_ROWS || a->K > FP4_MAX_K) return "M and N must be 2^30 at most, K 2^26";
   if (!fp4_format_ok(a->format)) return "format must be KREA_CUDA_FP4_MX or KREA_CUDA_FP4_NV";
   if (a->M == 0 || a->N == 0) return nullptr;
   if (a->K == 0) return "K must be positive";
@@ -90,7 +92,9 @@ inline const char* check_gemm_fp4(const krea_cuda_gemm_fp4_args* a) {
   if ((bias || a->epilogue == KREA_CUDA_EPI_RESID_GATE) && off16(a->vec)) return "vec must be 16-byte aligned";
   const int64_t cb = span(a->M, cols * es, (int64_t)a->ldc * es);
   if (overlap(a->C, cb, a->A, span(a->M, fp4_row_bytes(a->K), a->lda)) || overlap(a->C, cb, a->W, span(a->N, fp4_row_bytes(a->K), a->ldw)) ||
-      overlap(a->C, cb, a->a_scales, fp4_scale_bytes(a->format, a->M, a->K)) || overlap(a->C, cb, a->w_scales, fp4_scale_bytes(a->format, a->N, a->K)))
+      overlap(a->C, cb, a->a_scales, fp4_scale_bytes(a->format, a->M, a->K)) || overlap(a->C, cb, a->w_scales, fp4_scale_bytes(a->format, a->N, a->K)) ||
+      overlap(a->C, cb, a->a_tensor_scale, 4) || overlap(a->C, cb, a->w_tensor_scale, 4) ||
+      ((bias || a->epilogue == KREA_CUDA_EPI_RESID_GATE) && overlap(a->C, cb, a->vec, (int64_t)a->N * 4)))
     return "C overlaps an operand";
   return nullptr;
 }
@@ -99,7 +103,7 @@ constexpr int GATED_NORM_MAX_WIDTH = 32768;
 
 inline const char* check_gated_norm(const krea_cuda_gated_norm_args* a) {
   if (a->rows < 0 || a->width < 0) return "negative size";
-  if (a->rows > FP4_MAX_SIZE) return "rows must be 2^30 at most";
+  if (a->rows > FP4_MAX_ROWS) return "rows must be 2^30 at most";
   if (a->out < KREA_CUDA_OUT_BF16 || a->out > KREA_CUDA_OUT_FP4_NV) return "out must be one of KREA_CUDA_OUT_*";
   if (a->rows == 0 || a->width == 0) return nullptr;
   if (!a->x || !(a->x_out || a->h)) return "null tensor";
@@ -133,6 +137,10 @@ inline const char* check_gated_norm(const krea_cuda_gated_norm_args* a) {
   if (overlap(a->h, hs, a->x, xb) || overlap(a->h, hs, a->y, yb) || overlap(a->h, hs, a->x_out, xob)) return "h overlaps another tensor";
   if (overlap(a->h_scales, sb, a->x, xb) || overlap(a->h_scales, sb, a->y, yb) || overlap(a->h_scales, sb, a->x_out, xob) || overlap(a->h_scales, sb, a->h, hs))
     return "h_scales overlaps another tensor";
+  const int64_t vb = (a->mod_rows > 0 ? (R - 1) / a->mod_rows * a->mod_ld : 0) * 4 + W * 4;      // from the first vector to the end of the last
+  const struct { const void* p; int64_t n; } in[] = {{a->post, W * 4}, {a->gate, vb}, {a->mul, vb}, {a->add, vb}, {a->h_tensor_scale, 4}};
+  for (const auto& v : in)
+    if (overlap(a->x_out, xob, v.p, v.n) || overlap(a->h, hs, v.p, v.n) || overlap(a->h_scales, sb, v.p, v.n)) return "an output overlaps a vector";
   return nullptr;
 }
 

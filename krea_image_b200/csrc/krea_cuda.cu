@@ -277,6 +277,8 @@ int krea_cuda_sync(krea_cuda* h) {
   if (st != 0) {
     cudaMemsetAsync(h->status_dev, 0, 4, h->stream);
     cudaStreamSynchronize(h->stream);
+    if ((st & 0xFFu) >= 21u)      // sites of the 4-bit operators
+      return fail(h, KREA_CUDA_E_DEVICE, "a 4-bit operator gave up on a bounded wait: site %u, CTA %u", st & 0xFFu, (st >> 8) & 0xFFFu);
     return fail(h, KREA_CUDA_E_DEVICE, "attention kernel gave up on a bounded wait: site %u, query block %u, head %u",
                 st & 0xFFu, (st >> 8) & 0xFFFu, st >> 20);
   }

@@ -80,9 +80,10 @@ def _try(fn, cls, good, changes):
 def test_quantize_refusals(checks):
     good = dict(src=P[0], q=P[1], scales=P[2], tensor_scale=P[3], rows=5, K=70, ld=72, ldq=48, format=B.FP4_NV, transposed=0)
     _try(checks.fp4_quantize, B.Fp4QuantizeArgs, good, [
-        dict(rows=-1), dict(K=-1), dict(rows=(1 << 30) + 1), dict(K=(1 << 30) + 1, ld=0x7FFFFFF8, ldq=0x7FFFFFF0), dict(format=2), dict(format=-1), dict(src=None), dict(q=None), dict(scales=None),
+        dict(rows=-1), dict(K=-1), dict(rows=(1 << 30) + 1), dict(K=(1 << 26) + 1, ld=0x7FFFFFF8, ldq=0x7FFFFFF0), dict(format=2), dict(format=-1), dict(src=None), dict(q=None), dict(scales=None),
         dict(src=P[0] + 8), dict(q=P[1] + 4), dict(scales=P[2] + 2), dict(tensor_scale=P[3] + 2), dict(format=B.FP4_MX), dict(ld=68), dict(ld=76), dict(ldq=32),
-        dict(ldq=50), dict(transposed=1, rows=80), dict(q=P[0]), dict(scales=P[0] + 16), dict(scales=P[1]), dict(scales=P[1] + 4 * 48 + 32)])
+        dict(ldq=50), dict(transposed=1, rows=80), dict(q=P[0]), dict(scales=P[0] + 16), dict(scales=P[1]), dict(scales=P[1] + 4 * 48 + 32),
+        dict(tensor_scale=P[1] + 8), dict(tensor_scale=P[2])])
     for ch in (dict(rows=0, src=None), dict(K=0, q=None), dict(tensor_scale=None), dict(transposed=1, ld=8), dict(format=B.FP4_MX, tensor_scale=None)):
         assert checks.fp4_quantize(ctypes.byref(B.Fp4QuantizeArgs(**{**good, **ch}))) is None, ch
 
@@ -91,19 +92,19 @@ def test_dequantize_refusals(checks):
     good = dict(q=P[0], scales=P[1], tensor_scale=P[2], out=P[3], rows=5, K=70, ldq=48, ldo=72, format=B.FP4_NV)
     _try(checks.fp4_dequantize, B.Fp4DequantizeArgs, good, [
         dict(rows=-1), dict(K=-1), dict(format=7), dict(q=None), dict(scales=None), dict(out=None), dict(q=P[0] + 8), dict(scales=P[1] + 1), dict(out=P[3] + 2),
-        dict(tensor_scale=P[2] + 1), dict(format=B.FP4_MX), dict(ldq=32), dict(ldq=49), dict(ldo=70), dict(ldo=64), dict(out=P[0] + 32), dict(out=P[1])])
+        dict(tensor_scale=P[2] + 1), dict(format=B.FP4_MX), dict(ldq=32), dict(ldq=49), dict(ldo=70), dict(ldo=64), dict(out=P[0] + 32), dict(out=P[1]), dict(out=P[2])])
 
 
 def test_gemm_refusals(checks):
     good = dict(A=P[0], a_scales=P[1], W=P[2], w_scales=P[3], C=P[4], M=3, N=64, K=70, lda=48, ldw=64, ldc=64, format=B.FP4_NV, epilogue=B.EPI_BF16, vec=P[5],
                 a_tensor_scale=P[6], w_tensor_scale=P[7])
     _try(checks.gemm_fp4, B.GemmFp4Args, good, [
-        dict(M=-1), dict(N=-8), dict(K=-1), dict(K=0), dict(M=(1 << 30) + 1), dict(N=(1 << 30) + 8, ldc=(1 << 30) + 8), dict(K=0x7FFFFFFF, lda=0x7FFFFFF0, ldw=0x7FFFFFF0), dict(format=3), dict(A=None), dict(a_scales=None), dict(W=None), dict(w_scales=None), dict(C=None),
+        dict(M=-1), dict(N=-8), dict(K=-1), dict(K=0), dict(M=(1 << 30) + 1), dict(N=(1 << 30) + 8, ldc=(1 << 30) + 8), dict(K=(1 << 26) + 1, lda=0x7FFFFFF0, ldw=0x7FFFFFF0), dict(format=3), dict(A=None), dict(a_scales=None), dict(W=None), dict(w_scales=None), dict(C=None),
         dict(A=P[0] + 8), dict(a_scales=P[1] + 8), dict(W=P[2] + 8), dict(w_scales=P[3] + 8), dict(C=P[4] + 8), dict(a_tensor_scale=P[6] + 2), dict(w_tensor_scale=P[7] + 1),
         dict(format=B.FP4_MX), dict(lda=32), dict(lda=56), dict(ldw=32), dict(ldw=72), dict(N=60), dict(ldc=66), dict(ldc=56), dict(epilogue=B.EPI_SWIGLU, N=32),
         dict(epilogue=B.EPI_BIAS_BF16, vec=None), dict(epilogue=B.EPI_BIAS_F32, vec=P[5] + 4), dict(epilogue=B.EPI_RESID_GATE, vec=P[5] + 8), dict(C=P[0]), dict(C=P[2] + 64),
-        dict(C=P[1]), dict(C=P[3])])
-    for ch in (dict(M=0, A=None), dict(N=0), dict(epilogue=B.EPI_RESID_GATE, vec=None), dict(epilogue=B.EPI_SWIGLU, ldc=32)):
+        dict(C=P[1]), dict(C=P[3]), dict(C=P[6]), dict(C=P[7]), dict(epilogue=B.EPI_BIAS_BF16, C=P[5] + 16), dict(epilogue=B.EPI_RESID_GATE, C=P[5])])
+    for ch in (dict(M=0, A=None), dict(N=0), dict(epilogue=B.EPI_RESID_GATE, vec=None), dict(epilogue=B.EPI_SWIGLU, ldc=32), dict(C=P[5])):
         assert checks.gemm_fp4(ctypes.byref(B.GemmFp4Args(**{**good, **ch}))) is None, ch
 
 
@@ -116,7 +117,7 @@ def test_gated_norm_refusals(checks):
         dict(h_scales=None), dict(out=B.OUT_FP4_MX), dict(out=B.OUT_BF16, ld_h=40), dict(h_tensor_scale=P[5] + 2), dict(x=P[0] + 4), dict(y=P[1] + 2), dict(x_out=P[2] + 8), dict(h=P[3] + 8),
         dict(post=P[6] + 4), dict(gate=P[7] + 4), dict(mul=P[8] + 4), dict(add=P[9] + 4), dict(h_scales=P[4] + 4), dict(mod_rows=-1), dict(mod_ld=42), dict(mod_ld=-4),
         dict(eps=-1.0), dict(eps=float("nan")), dict(x_scale=float("inf")), dict(x_scale=float("nan")), dict(x_out=P[0]), dict(x_out=P[0] + 16, ld_xo=44), dict(x_out=P[1]), dict(h=P[0]),
-        dict(h=P[1] + 16), dict(h=P[2]), dict(h_scales=P[0]), dict(h_scales=P[3])])
+        dict(h=P[1] + 16), dict(h=P[2]), dict(h_scales=P[0]), dict(h_scales=P[3]), dict(h=P[6]), dict(h=P[5]), dict(x_out=P[7] + 160), dict(x_out=P[8] + 2 * 160 + 144), dict(h_scales=P[9])])
     for ch in (dict(rows=0, x=None), dict(x_out=P[0], ld_xo=44), dict(y=None, post=None, gate=None), dict(h=None, mul=None, h_scales=None), dict(out=B.OUT_F32, h_tensor_scale=None, ld_h=40),
                dict(out=B.OUT_BF16, h_tensor_scale=None, ld_h=40), dict(x_out=None), dict(y_f32=1, ld_y=44), dict(mod_rows=0, mod_ld=3), dict(eps=0.0)):
         assert checks.gated_norm(ctypes.byref(B.GatedNormArgs(**{**good, **ch}))) is None, ch

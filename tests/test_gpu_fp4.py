@@ -84,7 +84,7 @@ def _rows(rng, rows, K):
 
 @pytest.mark.parametrize("transposed", [False, True])
 @pytest.mark.parametrize("fmt,ts", [("mx", None), ("nv", None), ("nv", 0.0371), ("nv", 2.0 ** -5), ("nv", 7.40625 / 2688)])
-@pytest.mark.parametrize("rows,K", [(1, 1), (1, 16), (3, 31), (2, 32), (5, 33), (130, 70), (128, 256), (129, 257), (1, 6144), (300, 1000), (67, 2500)])
+@pytest.mark.parametrize("rows,K", [(1, 1), (1, 16), (3, 31), (2, 32), (5, 33), (130, 70), (128, 256), (129, 257), (1, 6144), (300, 1000), (67, 2500), (2000, 4200), (2500, 2600)])
 def test_quantise_is_exact(kc, rows, K, fmt, ts, transposed):
     bits = _rows(np.random.default_rng(rows * 31 + K), rows, K)
     t = 1.0 if ts is None else float(np.float32(ts))
@@ -290,6 +290,44 @@ def test_product_carries_what_is_not_finite(kp, M, N, K, fmt):
     want[M // 2, :] = np.nan
     want[:, N - 3] = np.nan
     assert np.array_equal(got, want, equal_nan=True)
+
+
+@pytest.mark.parametrize("epilogue", ["f32", "bf16", "swiglu", "resid_gate"])
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("M,N,K", [(2600, 4160, 520), (4700, 2112, 1300)])
+def test_many_tiles_a_worker(kp, M, N, K, fmt, epilogue):
+    """More tiles than CTA pairs and rows beyond one wave: accumulator, ring and output boxes are used again and again.  Sums
+    are exact in 32 bits (see above), so the plain epilogues are too; SwiGLU adds a sigmoid and a rounding."""
+    rng = np.random.default_rng(M + N)
+    qa, ca = _codes(rng, M, K, fmt, True)
+    qw, cw = _codes(rng, N, K, fmt, True)
+    A, As, va = _operand(qa, ca, fmt, K)
+    W, Ws, vw = _operand(qw, cw, fmt, K)
+    want = _dev(va) @ _dev(vw).T
+    vec = torch.from_numpy(rng.integers(-3, 4, N).astype(np.float32)).cuda()
+    cols = N // 2 if epilogue == "swiglu" else N
+    f32 = epilogue in ("f32", "resid_gate")
+    c = torch.full((M + 1, cols), 5.0, dtype=torch.float32 if f32 else torch.bfloat16, device="cuda")
+    kind = {"f32": B.EPI_F32, "bf16": B.EPI_BF16, "swiglu": B.EPI_SWIGLU, "resid_gate": B.EPI_RESID_GATE}[epilogue]
+    for _ in range(2):
+        c.fill_(5.0)
+        kp.gemm_fp4(A, As, W, Ws, c, M, N, K, A.shape[1], W.shape[1], cols, FMT[fmt], epilogue=kind, vec=vec if epilogue == "resid_gate" else None)
+    kp.wait()
+    assert (c[M] == 5).all()
+    got = c[:M]
+    if epilogue == "f32":
+        assert torch.equal(got, want.float())
+    elif epilogue == "bf16":
+        assert torch.equal(got, want.float().bfloat16())
+    elif epilogue == "resid_gate":                    # 3 * 2^20 + 5 in steps of 1/16: exact as well
+        assert torch.equal(got, (5 + vec.double() * want).float())
+    else:
+        pair = want.view(M, -1, 2, 32)
+        ref = (pair[:, :, 0] / (1 + torch.exp(-pair[:, :, 0])) * pair[:, :, 1]).reshape(M, cols)
+        # exp2's argument -g / ln 2 is below 128 where the sigmoid is not flushed to zero (at 2^-126): its two roundings of
+        # 2^-24 move the result by 128 * 2 * 2^-24 * ln 2 < 2^-16
+        flushed = (pair[:, :, 0] * pair[:, :, 1]).abs().reshape(M, cols) * 2.0 ** -126
+        assert ((got.double() - ref).abs() <= ref.abs() * (2.0 ** -8 + 2.0 ** -16) + flushed).all()
 
 
 def test_refusals_reach_the_caller(kc):

@@ -161,3 +161,55 @@ def test_refusals_reach_the_caller(kc):
     assert e.value.code == B.E_ARG
     kc.gated_norm(None, None, None, None, 0, 8, 8, 8, 8, 8)
     assert kc.launches == n0
+
+
+@pytest.mark.parametrize("pad", [4, 8])
+@pytest.mark.parametrize("out", ["bf16", "f32", "mx", "nv"])
+@pytest.mark.parametrize("rows,width,samples,y_f32,post", [(700, 264, 1, False, True), (900, 520, 3, True, True), (2001, 2568, 3, False, False), (61000, 16, 2, False, True), (299, 8200, 1, True, False),
+                                                           (300, 12304, 2, False, True)])
+def test_many_rows(kc, rows, width, samples, y_f32, post, out, pad):
+    """Enough rows that a CTA takes several, samples that end within its share, and rows that start on 16 bytes but not on 32
+    (pad 4) as well as on 32 (pad 8): chosen rows against float64, and 4-bit rows against the bf16 rows of the same call."""
+    pad_y = 8 if pad == 4 and not y_f32 else pad        # bf16 rows start on 16 bytes all the same
+    rng = np.random.default_rng(rows + width)
+    per = -(-rows // samples)
+    x, y = rng.standard_normal((rows, width), dtype=np.float32), rng.standard_normal((rows, width), dtype=np.float32)
+    if not y_f32:
+        y = synth.bf16_bits_to_f32(synth.f32_to_bf16_bits(y)).reshape(y.shape)
+    vec = lambda m, d: (m + d * rng.standard_normal((samples, width))).astype(np.float32)  # noqa: E731
+    w, gate, mul, add = vec(1, .3)[0] if post else None, vec(0, .8), vec(1, .3), vec(0, .2)
+    X, Y = _wide(x, pad), _wide(y, pad_y, torch.float32 if y_f32 else torch.bfloat16)
+    D = [None if v is None else _dev(v) for v in (w, gate, mul, add)]
+
+    def run(kind):
+        XO = torch.full((rows, width + pad), -7.0, device="cuda")
+        S = None
+        if kind in ("mx", "nv"):
+            H = torch.full((rows, ops.fp4_row_bytes(width) + 16), 0xA5, dtype=torch.uint8, device="cuda")
+            S = torch.full((ops.fp4_scale_bytes(B.FP4_MX if kind == "mx" else B.FP4_NV, rows, width),), 0xA5, dtype=torch.uint8, device="cuda")
+        else:
+            H = torch.full((rows, width + 8), -7.0, dtype=torch.bfloat16 if kind == "bf16" else torch.float32, device="cuda")
+        kc.gated_norm(X, Y, XO, H, rows, width, width + pad, width + pad_y, width + pad, H.shape[1], post=D[0], gate=D[1], mul=D[2], add=D[3], x_scale=0.5, eps=EPS,
+                      mod_rows=per, mod_ld=width, y_f32=y_f32, out=OUT[kind], h_scales=S)
+        kc.wait()
+        assert (XO[:, width:] == -7).all()
+        return XO[:, :width], H, S
+
+    XO, H, S = run(out)
+    picks = sorted({0, 1, 127, per - 1, min(per, rows - 1), rows // 2, rows - 129, rows - 1})
+    if out in ("mx", "nv"):
+        rb = ops.fp4_row_bytes(width)
+        XB, HB, _ = run("bf16")
+        assert torch.equal(XO, XB) and (H[:, rb:] == 0xA5).all()
+        want_q, want_s = fp4_np.quantise(HB[:, :width].double().cpu().numpy(), out)
+        assert np.array_equal(H[:, :rb].cpu().numpy(), fp4_np.pack(want_q, width))
+        assert np.array_equal(S.cpu().numpy(), fp4_np.lay_out_scales(want_s, out, width))
+        return
+    assert (H[:, width:] == -7).all()
+    f = lambda v: v.astype(np.float64)  # noqa: E731
+    at = np.array(picks) // per
+    for i, r in enumerate(picks):
+        a = at[i]
+        want_x, want_h = fp4_np.gated_norm(f(x[r:r + 1]), f(y[r:r + 1]), None if w is None else f(w), f(gate[a:a + 1]), f(mul[a:a + 1]), f(add[a:a + 1]), 0.5, EPS, 0)
+        yr = y[r:r + 1] if w is None else y[r:r + 1] / np.sqrt((f(y[r:r + 1]) ** 2).mean(1, keepdims=True) + EPS) * w
+        _check(XO[r:r + 1].cpu().numpy(), H[r:r + 1, :width].double().cpu().numpy(), want_x, want_h, 0.5 * x[r:r + 1], y[r:r + 1], mul[a:a + 1], add[a:a + 1], width, out, yr, gate[a:a + 1])
