@@ -6,8 +6,8 @@
 //
 // HBM-bound: 2 bytes read and 0.53 (MX) or 0.56 (NV) written per value.  A warp takes the four blocks that share a
 // 4-byte word of scales from rows 32 apart, which makes its scale bytes one contiguous piece (16 or 32 bytes) and its
-// reads whole 128-byte lines.  Measured at 4608 x 16384: MX 32 us (92 % of the copy bandwidth), NV 42 us (71 %: the
-// instructions of the scales), back to bf16 34 and 39 us (88 and 76 %).
+// reads whole 128-byte lines.  Measured at 4608 x 16384: MX 30.1 us (98 % of the copy bandwidth), NV 39 us (77 %: the
+// instructions of the scales), back to bf16 32.6 and 34.2 us (91 and 88 %).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -39,28 +39,32 @@ __device__ __forceinline__ void load16(const __nv_bfloat16* src, int left, bool 
   }
 }
 
+// How a CTA's 8 warps lie on (column, row) items: 2^cols_log2 of them beside one another, the others on further rows.  Row items
+// go on in steps of the grid's height, so that no index is divided.
+struct Fp4Shape {
+  int cols, cols_log2;      // column items; log2 of how many a CTA has
+  int row_items;
+};
+
 template <bool MX>
-__global__ void __launch_bounds__(FQ_THREADS) fp4_quantize_rows_kernel(const Fp4QuantParams p) {
+__global__ void __launch_bounds__(FQ_THREADS) fp4_quantize_rows_kernel(const Fp4QuantParams p, const Fp4Shape z) {
   constexpr int LANES = MX ? 8 : 4;              // lanes of a row: 16 values each, four blocks together
-  constexpr int GROUP = LANES * 16;              // values of those four blocks
-  constexpr int RUNS = MX ? 32 : 16;             // warp items that cover the 128 rows of a scale tile
+  constexpr int GROUP = LANES * 16;              // values of those four blocks; a column item is two such groups
+  constexpr int RUNS = MX ? 32 : 16;             // row items that cover the 128 rows of a scale tile
   const int64_t chunks = (p.K + 255) / 256;
-  const int groups = (int)chunks * (256 / GROUP);
-  const int64_t items = (int64_t)((p.rows + 127) / 128) * RUNS * (groups / 2);          // two groups at a time
-  const int lane = threadIdx.x & 31, in_row = lane % LANES, rr = lane / LANES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, in_row = lane % LANES, rr = lane / LANES;
   griddep_wait();
   __shared__ NvTable nv;
   if constexpr (!MX) {
     if (threadIdx.x < 128) nv_table_fill(nv, p.tensor_scale ? __ldg(p.tensor_scale) : 1.f, threadIdx.x);
     __syncthreads();
   }
-  const int64_t step = (int64_t)gridDim.x * (FQ_THREADS / 32);
   const bool wide = (((uintptr_t)p.src | (uintptr_t)(p.ld * 2)) & 31u) == 0;
-  for (int64_t it = (int64_t)blockIdx.x * (FQ_THREADS / 32) + (threadIdx.x >> 5); it < items; it += step) {
-    const int g = (int)(it % (groups / 2)) * 2;
-    const int64_t tr = it / (groups / 2);
-    const int run = (int)(tr % RUNS);
-    const int row = (int)(tr / RUNS) * 128 + (rr & 3) * 32 + (MX ? run : run * 2 + (rr >> 2));
+  const int g = (((int)blockIdx.x << z.cols_log2) + (warp & ((1 << z.cols_log2) - 1))) * 2, rows_cta = 8 >> z.cols_log2;
+  if (g >= 2 * z.cols) return;
+  for (int tr = (int)blockIdx.y * rows_cta + (warp >> z.cols_log2); tr < z.row_items; tr += (int)gridDim.y * rows_cta) {
+    const int run = tr % RUNS;
+    const int row = tr / RUNS * 128 + (rr & 3) * 32 + (MX ? run : run * 2 + (rr >> 2));
     const __nv_bfloat16* src = p.src + (int64_t)row * p.ld;
     uint32_t w[2][8];
 #pragma unroll
@@ -108,7 +112,19 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp4_quantize_cols_kernel(const 
   __shared__ NvTable nv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kt = (p.K + 255) / 256 * 2, nt = (p.rows + FT_N - 1) / FT_N;       // padding included: its scales are written too
-  const int64_t items = (int64_t)kt * nt;
+  // tiles in steps of the grid, rows fastest
+  struct Place {
+    int k, n;
+  };
+  const int step_k = (int)gridDim.x / nt, step_n = (int)gridDim.x - step_k * nt;
+  const auto next = [&](Place& t) {
+    t.k += step_k;
+    t.n += step_n;
+    if (t.n >= nt) t.n -= nt, t.k++;
+  };
+  Place at = {(int)blockIdx.x / nt, 0}, ahead;
+  at.n = (int)blockIdx.x - at.k * nt;
+  ahead = at;
   if (threadIdx.x == 0) {
     for (int s = 0; s < FT_STAGES; s++) mbar_init(&full[s], 1);
     abort_word[0] = 0u;
@@ -119,26 +135,28 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp4_quantize_cols_kernel(const 
     if (threadIdx.x < 128) nv_table_fill(nv, p.tensor_scale ? __ldg(p.tensor_scale) : 1.f, threadIdx.x);
   }
   __syncthreads();
-  const auto request = [&](int64_t item, int s) {
-    mbar_arrive_expect_tx(&full[s], FT_TILE);
-    tma_load_3d(smem + s * FT_TILE, &tm, &full[s], (int)(item % nt) * FT_N, (int)(item / nt) * FT_K, 0);
+  const auto request = [&](int s) {                // the next tile not asked for yet, if there is one
+    if (ahead.k < kt) {
+      mbar_arrive_expect_tx(&full[s], FT_TILE);
+      tma_load_3d(smem + s * FT_TILE, &tm, &full[s], ahead.n * FT_N, ahead.k * FT_K, 0);
+      next(ahead);
+    }
   };
   if (threadIdx.x == 0) {
-    for (int s = 0; s < FT_STAGES; s++)
-      if (blockIdx.x + (int64_t)s * gridDim.x < items) request(blockIdx.x + (int64_t)s * gridDim.x, s);
+    for (int s = 0; s < FT_STAGES; s++) request(s);
   }
   const int g = warp & 3, n2 = (warp >> 2) * 32 + lane;       // 32 k from 32 g on, output rows 2 n2 and 2 n2 + 1 of the tile
   int s = 0;
   uint32_t phase = 0;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int n0 = (int)(item % nt) * FT_N, k0 = (int)(item / nt) * FT_K;
+  for (; at.k < kt; next(at)) {
+    const int n0 = at.n * FT_N, k0 = at.k * FT_K;
     if (__syncthreads_or(!mbar_wait(&full[s], phase, abort_word, SITE_QUANT_FULL))) break;
     const uint32_t* tile = (const uint32_t*)(smem + s * FT_TILE);
     uint32_t t[32];
 #pragma unroll
     for (int i = 0; i < 32; i++) t[i] = tile[(g * 32 + i) * (FT_N / 2) + n2];
     __syncthreads();                                 // the stage has been read, and the last tile's results have left
-    if (threadIdx.x == 0 && item + (int64_t)FT_STAGES * gridDim.x < items) request(item + (int64_t)FT_STAGES * gridDim.x, s);
+    if (threadIdx.x == 0) request(s);
     if (++s == FT_STAGES) s = 0, phase ^= 1u;
 #pragma unroll
     for (int half = 0; half < 2; half++) {
@@ -189,15 +207,27 @@ cudaError_t launch_fp4_quantize_cols(const CUtensorMap& tm, const Fp4QuantParams
   return launch_kernel(k, dim3((unsigned)(items < 2 * sms ? items : 2 * sms)), FT_THREADS, FT_SMEM, stream, pdl, 1, false, tm, p);
 }
 
+// the grid for these items, `most` CTAs at most
+static dim3 shape_grid(int64_t cols, int64_t row_items, int64_t most, Fp4Shape* z) {
+  z->cols = (int)cols;
+  z->row_items = (int)row_items;
+  z->cols_log2 = 0;
+  while (z->cols_log2 < 3 && (1ll << z->cols_log2) < cols) z->cols_log2++;
+  const int64_t x = (cols + (1ll << z->cols_log2) - 1) >> z->cols_log2, rows_cta = 8 >> z->cols_log2;
+  int64_t y = (row_items + rows_cta - 1) / rows_cta;
+  if (x * y > most) y = most / x;
+  if (y < 1) y = 1;
+  if (y > 65535) y = 65535;
+  return dim3((unsigned)x, (unsigned)y);
+}
+
 cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, bool pdl, cudaStream_t stream) {
   if (p.rows <= 0 || p.K <= 0) return cudaSuccess;
   const int64_t tiles = (p.rows + 127) / 128, chunks = (p.K + 255) / 256;
-  const int64_t items = tiles * (p.mx ? 32 : 16 * 2) * chunks;
-  int64_t blocks = (items + FQ_THREADS / 32 - 1) / (FQ_THREADS / 32);
-  // MX: two rounds of the CTAs that fit.  NV: one round, since each fills its table first (4608 x 16384: 42.2 us, 45.2 with MX's)
-  const int64_t most = 148 * (p.mx ? 16 : 4);
-  if (blocks > most) blocks = most;
-  return launch_kernel(p.mx ? fp4_quantize_rows_kernel<true> : fp4_quantize_rows_kernel<false>, dim3((unsigned)blocks), FQ_THREADS, 0, stream, pdl, 1, false, p);
+  Fp4Shape z;
+  // MX: two rounds of the CTAs that fit.  NV: one round, since each fills its table first (4608 x 16384: 39 us, 45 with MX's)
+  const dim3 grid = shape_grid(chunks * (p.mx ? 1 : 2), tiles * (p.mx ? 32 : 16), 148 * (p.mx ? 16 : 4), &z);
+  return launch_kernel(p.mx ? fp4_quantize_rows_kernel<true> : fp4_quantize_rows_kernel<false>, grid, FQ_THREADS, 0, stream, pdl, 1, false, p, z);
 }
 
 // ---- back to bf16: bf16(e2m1 * block scale * tensor scale), rounded once from f32 ----
@@ -212,11 +242,12 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_dequantize_kernel(const Fp4Deq
   const int64_t chunks = (p.K + 255) / 256;
   const int per_row = (p.K + 15) / 16;                 // 16 values a thread
   const int64_t items = (int64_t)p.rows * per_row, step = (int64_t)gridDim.x * FQ_THREADS;
+  const bool narrow = items <= 0xFFFFFFFFll;            // a 64-bit division costs as much as the rest
   const bool wide = (((uintptr_t)p.out | (uintptr_t)(p.ldo * 2)) & 31u) == 0;
   griddep_wait();
   const float ts = MX || !p.tensor_scale ? 1.f : __ldg(p.tensor_scale);
   for (int64_t it = (int64_t)blockIdx.x * FQ_THREADS + threadIdx.x; it < items; it += step) {
-    const int row = (int)(it / per_row), k0 = (int)(it - (int64_t)row * per_row) * 16;
+    const int row = narrow ? (int)((uint32_t)it / (uint32_t)per_row) : (int)(it / per_row), k0 = (int)(it - (int64_t)row * per_row) * 16;
     const uint2 q = __ldg((const uint2*)(p.q + (int64_t)row * p.ldq + (k0 >> 1)));
     const uint32_t code = __ldg(p.scales + scale_offset<MX>(row, MX ? k0 >> 5 : k0 >> 4, chunks));
     float s;

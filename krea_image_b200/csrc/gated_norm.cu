@@ -177,8 +177,14 @@ __global__ void __maxnreg__(REGS) gated_norm_kernel(const GatedNormParams p) {
     }
     return r;
   };
+  int64_t mod = 0;                 // where the row's vectors start
+  unsigned until = p.mod_rows > 0 ? 0u : 0xFFFFFFFFu;      // first row that has others
   for (int it = 0; row < (unsigned)p.rows; it ^= 1) {
-    const int64_t mod = p.mod_rows > 0 ? (int64_t)(row / (unsigned)p.mod_rows) * p.mod_ld : 0;
+    if (row >= until) {
+      const unsigned sample = row / (unsigned)p.mod_rows;
+      mod = (int64_t)sample * p.mod_ld;
+      until = (sample + 1u) * (unsigned)p.mod_rows;
+    }
     const float *gate = p.gate ? p.gate + mod : nullptr, *mul = p.h ? p.mul + mod : nullptr, *add = p.add ? p.add + mod : nullptr;
     F8 v[HOLD], w[AHEAD ? HOLD : 1], w2[AHEAD ? HOLD : 1];
     if constexpr (AHEAD) {
