@@ -61,11 +61,17 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t saddr16) {
   else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 
+// Asked for at the kernel's start and not where the compiler would put it, next to the use: a memory latency at the end of
+// every launch.
 __device__ __forceinline__ float tensor_scale(const Fp4GemmParams& p) {
-  float s = 1.f;
-  if (p.a_ts) s *= __ldg(p.a_ts);
-  if (p.w_ts) s *= __ldg(p.w_ts);
-  return s;
+  float a = 1.f, w = 1.f;
+  if (p.a_ts) asm volatile("ld.global.f32 %0, [%1];" : "=f"(a) : "l"(p.a_ts));
+  if (p.w_ts) asm volatile("ld.global.f32 %0, [%1];" : "=f"(w) : "l"(p.w_ts));
+  return a * w;
+}
+// An earlier kernel gave up on a wait: this one does nothing.  Looked at by a warp that has nothing else to do then.
+__device__ __forceinline__ void check_status(const Fp4GemmParams& p, volatile uint32_t* abort_word) {
+  if (p.status != nullptr && *(volatile uint32_t*)p.status != 0u) abort_word[0] = 0xFFu;
 }
 __device__ __forceinline__ float gelu_tanh(float x) { return 0.5f * x * (1.0f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x))); }
 
@@ -158,26 +164,38 @@ __device__ __forceinline__ void pair_store(const Fp4GemmParams& p, const CUtenso
     }
     return;
   }
+  // one path a kind, each without the others' instructions between its own: a cold launch fetches them once, in order
+  const auto bf16_boxes = [&](auto after) {
 #pragma unroll
-  for (int c0 = 0; c0 < 128; c0 += 64) {
-    if (col0 + c0 >= p.N) break;
-    begin();
+    for (int c0 = 0; c0 < 128; c0 += 64) {
+      if (col0 + c0 >= p.N) break;
+      begin();
 #pragma unroll
-    for (int q = 0; q < 8; q++) {
-      const int c = c0 + q * 8;
-      float f[8];
+      for (int q = 0; q < 8; q++) {
+        const int c = c0 + q * 8;
+        float f[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) f[e] = acc(c + e);
-      if (p.epi == KREA_CUDA_EPI_BIAS_BF16 && col0 + c < p.N) {
-        const float4 a = __ldg((const float4*)(p.vec + col0 + c)), b = __ldg((const float4*)(p.vec + col0 + c) + 1);
-        f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
-      } else if (p.epi == KREA_CUDA_EPI_GELU) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) f[e] = gelu_tanh(f[e]);
+        for (int e = 0; e < 8; e++) f[e] = acc(c + e);
+        after(f, col0 + c);
+        put(q, pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
       }
-      put(q, pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+      send(col0 + c0);
     }
-    send(col0 + c0);
+  };
+  if (p.epi == KREA_CUDA_EPI_BF16) {
+    bf16_boxes([](float*, int) {});
+  } else if (p.epi == KREA_CUDA_EPI_BIAS_BF16) {
+    bf16_boxes([&](float* f, int col) {
+      if (col < p.N) {
+        const float4 a = __ldg((const float4*)(p.vec + col)), b = __ldg((const float4*)(p.vec + col) + 1);
+        f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+      }
+    });
+  } else {
+    bf16_boxes([](float* f, int) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[e] = gelu_tanh(f[e]);
+    });
   }
 }
 // C (f32) += vec * acc for 128 columns of a row
@@ -262,10 +280,11 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const uint32_t tmem_base = *tmem_slot, sf_base = tmem_base + (uint32_t)rows_acc_cols(TN);
   griddep_wait();
   griddep_launch();
+  if (threadIdx.x == 64) check_status(p, abort_word);
+  const float alpha = tensor_scale(p);
 
   if (warp == 0) {
     if (lane == 0) {
-      if (p.status != nullptr && *(volatile uint32_t*)p.status != 0u) abort_word[0] = 0xFFu;      // an earlier kernel gave up: do nothing
       int s = 0, done = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1 && *abort_word == 0u; kb++, done++) {
@@ -350,7 +369,6 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   // parts added in rank order, 8 columns of a row at a time
   const bool swiglu = p.epi == KREA_CUDA_EPI_SWIGLU;
   const int units_row = swiglu ? 8 : 16, r0 = (int)rank * share, mine = min(rows - r0, share);
-  const float alpha = tensor_scale(p);
   const bool live = *abort_word == 0u;
   for (int u = threadIdx.x; live && u < mine * units_row; u += ROWS_THREADS) {
     const int r = u / units_row, uc = u % units_row;
@@ -462,8 +480,6 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 
   // tile t -> origin: groups of group_m row blocks x all column blocks, row block fastest, so that the pairs running
   // together share a few rows of both operands and a group's slice of A stays in L2
-  griddep_wait();
-  griddep_launch();
   auto tile_origin = [&](int t, int& m0, int& n0) {
     const int per_group = p.group_m * nt;
     const int g = t / per_group, first = g * p.group_m;
@@ -472,13 +488,16 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     m0 = (first + local % gm) * TILE_M + (int)rank * 128;     // this CTA's rows of the tile
     n0 = (local / gm) * BN;
   };
+  int m0 = 0, n0 = 0;
+  tile_origin(worker, m0, n0);       // the divisions of the first tile are done before the wait
+  griddep_wait();
+  griddep_launch();
+  if (threadIdx.x == 96) check_status(p, abort_word);
   if (warp == 0) {
     if (lane == 0) {
-      if (p.status != nullptr && *(volatile uint32_t*)p.status != 0u) abort_word[0] = 0xFFu;      // an earlier kernel gave up: do nothing
       uint32_t n = 0;
       for (int t = worker; t < tiles && *abort_word == 0u; t += workers) {
-        int m0, n0;
-        tile_origin(t, m0, n0);
+        if (t != worker) tile_origin(t, m0, n0);
         for (int kb = 0; kb < kblocks; kb++, n++) {
           const int s = n % STAGES;
           if (!mbar_wait(&empty[s], ((n / STAGES) & 1) ^ 1, abort_word, SITE_EMPTY)) break;
@@ -545,8 +564,7 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const float alpha = tensor_scale(p);
     int it = 0;
     for (int t = worker; t < tiles; t += workers, it++) {
-      int m0, n0;
-      tile_origin(t, m0, n0);
+      if (t != worker) tile_origin(t, m0, n0);
       if (!mbar_wait(acc_full, it & 1, abort_word, SITE_ACC_FULL)) break;
       tc_fence_after();
       uint32_t v[128];
