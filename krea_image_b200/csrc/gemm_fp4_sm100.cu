@@ -340,7 +340,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int rows = min(TN, p.M - m0), share = (rows + (int)split - 1) / (int)split;
   bool done = true;
   if (warp >= 2) {
-    done = mbar_wait(acc_full, 0, abort_word, SITE_ACC_FULL);
+    done = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_word, SITE_ACC_FULL));      // what follows takes whole warps
     tc_fence_after();
   }
   __syncwarp();
@@ -563,9 +563,10 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const uint32_t src = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
     const float alpha = tensor_scale(p);
     int it = 0;
+    bool arrived = false;
     for (int t = worker; t < tiles; t += workers, it++) {
       if (t != worker) tile_origin(t, m0, n0);
-      if (!mbar_wait(acc_full, it & 1, abort_word, SITE_ACC_FULL)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full, it & 1, abort_word, SITE_ACC_FULL))) break;      // what follows takes whole warps
       tc_fence_after();
       uint32_t v[128];
 #pragma unroll
@@ -574,21 +575,30 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster_relaxed(mapa(smem_u32(acc_empty), 0));
+      const bool last = t + workers >= tiles;
+      if (last) {                  // this warp has no more business with the other CTA
+        cluster_arrive();
+        arrived = true;
+      }
       const int row0 = m0 + quarter * 32, col0 = n0 + half * 128;
       if (row0 >= p.M || col0 >= p.N) continue;
       if (p.epi == KREA_CUDA_EPI_RESID_GATE) {
         if (row0 + lane < p.M) pair_add(p, v, row0 + lane, col0, alpha);
       } else {
-        // after a worker's last tile the stages are free: every box of a warp has a place of its own there
-        const bool last = t + workers >= tiles;
         // All pairs end their tiles at about the same time, and 64 KB from every SM at once hold up the loads of the next ones:
         // the warps take turns over the next tile's products (4608 x 15360 x 6144: 183 -> 177 us NV, 176 -> 170 us MX)
         if (!last) __nanosleep((uint32_t)((warp - 4) * kblocks * PACE_NS));
+        // after a worker's last tile the stages are free: every box of a warp has a place of its own there
         pair_store(p, tmC, v, row0, col0, alpha, last ? smem + (warp - 4) * 4 * C::OUT_BYTES : out_smem + (warp - 4) * C::OUT_BYTES, last, lane);
       }
     }
     if (lane == 0) tma_store_wait_read();      // the last box has left shared memory
     __syncwarp();
+    if (!arrived) cluster_arrive();
+  }
+  if (warp < 4) {
+    __syncwarp();
+    cluster_arrive();
   }
 
   // nobody leaves or frees tensor memory while the peer may still read this CTA's shared memory, signal its barriers or
@@ -596,7 +606,7 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   tc_fence_before();
   __syncwarp();
   __syncthreads();
-  cluster_sync_all();
+  cluster_wait();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc2(tmem_base, C::TMEM_COLS);
