@@ -24,7 +24,7 @@
 namespace krea {
 
 namespace fp4g {
-enum : uint32_t { SITE_FULL = 21, SITE_EMPTY = 22, SITE_ACC_FULL = 23, SITE_ACC_EMPTY = 24 };
+enum : uint32_t { SITE_FULL = 21, SITE_EMPTY = 22, SITE_ACC_FULL = 23, SITE_ACC_EMPTY = 24, SITE_PARTS = 25 };
 constexpr int KB = 256;                              // values of K a stage: one 128-byte row of packed values
 constexpr int ROW_TILE_BYTES = 128 * 128;            // 128 rows of a stage
 __host__ __device__ constexpr int scale_chunk(bool mx) { return mx ? 1024 : 2048; }   // scale bytes of 128 rows x 256 values
@@ -61,14 +61,15 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t saddr16) {
   else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 
-// Asked for at the kernel's start and not where the compiler would put it, next to the use: a memory latency at the end of
-// every launch.
-__device__ __forceinline__ float tensor_scale(const Fp4GemmParams& p) {
+// Both tensor scales.  Asked for at the kernel's start and not where the compiler would put it, next to the use: a memory
+// latency at the end of every launch.  Multiplied at the use: before that nobody waits for them.
+struct TensorScales {
   float a = 1.f, w = 1.f;
-  if (p.a_ts) asm volatile("ld.global.f32 %0, [%1];" : "=f"(a) : "l"(p.a_ts));
-  if (p.w_ts) asm volatile("ld.global.f32 %0, [%1];" : "=f"(w) : "l"(p.w_ts));
-  return a * w;
-}
+  __device__ __forceinline__ explicit TensorScales(const Fp4GemmParams& p) {
+    if (p.a_ts) asm volatile("ld.global.f32 %0, [%1];" : "=f"(a) : "l"(p.a_ts));
+    if (p.w_ts) asm volatile("ld.global.f32 %0, [%1];" : "=f"(w) : "l"(p.w_ts));
+  }
+};
 // An earlier kernel gave up on a wait: this one does nothing.  Looked at by a warp that has nothing else to do then.
 __device__ __forceinline__ void check_status(const Fp4GemmParams& p, volatile uint32_t* abort_word) {
   if (p.status != nullptr && *(volatile uint32_t*)p.status != 0u) abort_word[0] = 0xFFu;
@@ -223,18 +224,6 @@ constexpr int ROWS_MAX_STAGES = 8;
 constexpr int ROWS_THREADS = 192;   // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 }  // namespace fp4g
 
-// up to 32 rows of one column, 512 bytes apart, in this CTA's shared memory or another's
-template <bool CLUSTER>
-__device__ __forceinline__ void put_rows(uint32_t at, const uint32_t* v, int n) {
-#pragma unroll
-  for (int e = 0; e < 32; e++) {
-    if (e < n) {
-      if constexpr (CLUSTER) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at + e * 512), "r"(v[e]) : "memory");
-      else asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + e * 512), "r"(v[e]) : "memory");
-    }
-  }
-}
-
 template <bool MX>
 __global__ void __launch_bounds__(fp4g::ROWS_THREADS)
 gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs, const __grid_constant__ CUtensorMap tmW,
@@ -248,7 +237,8 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   uint64_t* full = (uint64_t*)(smem + STAGES * STAGE_BYTES);
   uint64_t* empty = full + ROWS_MAX_STAGES;
   uint64_t* acc_full = empty + ROWS_MAX_STAGES;
-  uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
+  uint64_t* received = acc_full + 1;                     // the other CTAs' parts of this CTA's rows have arrived
+  uint32_t* tmem_slot = (uint32_t*)(received + 1);
   volatile uint32_t* abort_word = (volatile uint32_t*)(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -267,6 +257,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
+    mbar_init(received, 1);
     abort_word[0] = abort_word[1] = 0u;
     fence_mbar_init();
   }
@@ -281,7 +272,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   griddep_wait();
   griddep_launch();
   if (threadIdx.x == 64) check_status(p, abort_word);
-  const float alpha = tensor_scale(p);
+  const TensorScales scales(p);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -333,45 +324,64 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (leader) umma_commit(acc_full);
     __syncwarp();
   }
-  // Each CTA of the cluster finishes an equal share of the tile's rows.  The parts of a row go straight from tensor memory
-  // to the shared memory of the CTA that finishes it, as [CTA they come from][row][128 columns of C] f32, over its
-  // stages: stores have no latency to wait for, and after them nobody touches another CTA's memory.
+  // Each CTA of the cluster finishes an equal share of the tile's rows.  The tile goes from tensor memory to this CTA's shared
+  // memory, over the stages, as [row][128 columns of C] f32; bulk copies take the other CTAs' rows to them, into
+  // [CTA they come from][row][128 columns] behind their own tile.
   float* part = (float*)smem;
+  float* parts = part + TN * 128;
   const int rows = min(TN, p.M - m0), share = (rows + (int)split - 1) / (int)split;
+  const auto rows_of = [&](int q) { return max(0, min(rows - q * share, share)); };
+  const int r0 = (int)rank * share, mine = rows_of((int)rank);
+  if (split > 1 && threadIdx.x == 0 && mine > 0) mbar_arrive_expect_tx(received, (split - 1) * (uint32_t)mine * 512u);
   bool done = true;
   if (warp >= 2) {
     done = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_word, SITE_ACC_FULL));      // what follows takes whole warps
     tc_fence_after();
   }
   __syncwarp();
-  if (split > 1) cluster_sync_all();         // no CTA's stages are in use any more
-  if (warp >= 2 && done) {
+  if (split > 1) cluster_arrive();           // nothing uses this CTA's stages any more
+  if (warp >= 2) {
     const int quarter = warp & 3;
-    for (uint32_t q = 0; q < split; q++) {   // CTA q's rows
-      const int first = (int)q * share, n = min(rows - first, share);
-      const uint32_t here = smem_u32(part + (int)rank * share * 128 + quarter * 32 + lane), to = split > 1 ? mapa(here, q) : here;
+    if (done) {
 #pragma unroll 1
-      for (int c0 = 0; c0 < n; c0 += 32) {
+      for (int c0 = 0; c0 < rows; c0 += 32) {
         uint32_t v[32];
-        tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(first + c0), v);
+        tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c0, v);
         tmem_wait_ld();
-        const uint32_t at = to + (uint32_t)c0 * 512u;
-        if (split > 1) put_rows<true>(at, v, n - c0);
-        else put_rows<false>(at, v, n - c0);
+        const uint32_t at = smem_u32(part + c0 * 128 + quarter * 32 + lane);
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+          if (c0 + e < rows) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + e * 512), "r"(v[e]) : "memory");
       }
     }
+    fence_proxy_async_smem();                // the copies read what was stored
     tc_fence_before();
   }
   __syncwarp();
-  if (split > 1) cluster_sync_all();
-  else __syncthreads();
+  __syncthreads();
+  bool live = *abort_word == 0u;
+  if (split > 1) {
+    cluster_wait();
+    if (threadIdx.x == 0 && live) {
+      for (uint32_t q = 0; q < split; q++) {
+        const int n = rows_of((int)q);
+        if (q != rank && n > 0) {
+          const uint32_t dst = mapa(smem_u32(parts + (int)(rank < q ? rank : rank - 1) * share * 128), q);
+          bulk_copy_cluster(dst, smem_u32(part + (int)q * share * 128), (uint32_t)n * 512u, mapa(smem_u32(received), q));
+        }
+      }
+    }
+    if (mine > 0) live = mbar_wait(received, 0, abort_word, SITE_PARTS) && live;
+    __syncwarp();
+    cluster_arrive();                        // this CTA has what the others sent
+  }
 
   // parts added in rank order, 8 columns of a row at a time
   const bool swiglu = p.epi == KREA_CUDA_EPI_SWIGLU;
-  const int units_row = swiglu ? 8 : 16, r0 = (int)rank * share, mine = min(rows - r0, share);
-  const bool live = *abort_word == 0u;
-  for (int u = threadIdx.x; live && u < mine * units_row; u += ROWS_THREADS) {
-    const int r = u / units_row, uc = u % units_row;
+  const int units_log2 = swiglu ? 3 : 4;
+  const float alpha = scales.a * scales.w;
+  for (int u = threadIdx.x; live && u < mine << units_log2; u += ROWS_THREADS) {
+    const int r = u >> units_log2, uc = u & ((1 << units_log2) - 1);
     const int c = swiglu ? (uc >> 2) * 64 + (uc & 3) * 8 : uc * 8;       // first of the tile's columns (SwiGLU: of the gate's)
     if (n0 + c >= p.N) continue;
     float f[8], g[8];
@@ -379,8 +389,8 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] = 0.f;
       for (uint32_t q = 0; q < split; q++) {
-        const float4* at = (const float4*)(part + ((int)q * share + r) * 128 + col);
-        const float4 x = at[0], y = at[1];
+        const float* from = q == rank ? part + (r0 + r) * 128 : parts + ((int)(q < rank ? q : q - 1) * share + r) * 128;
+        const float4 x = *(const float4*)(from + col), y = *(const float4*)(from + col + 4);
         o[0] += x.x; o[1] += x.y; o[2] += x.z; o[3] += x.w; o[4] += y.x; o[5] += y.y; o[6] += y.z; o[7] += y.w;
       }
 #pragma unroll
@@ -398,6 +408,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
   __syncwarp();
   __syncthreads();
+  if (split > 1) cluster_wait();             // the others have what this CTA sent
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, TMEM_COLS);
@@ -561,7 +572,8 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     // with them: the tensor cores go on while the stores are under way.
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t src = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
-    const float alpha = tensor_scale(p);
+    const TensorScales scales(p);
+    const float alpha = scales.a * scales.w;
     int it = 0;
     bool arrived = false;
     for (int t = worker; t < tiles; t += workers, it++) {
@@ -679,6 +691,8 @@ Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force) {
   plan.stages = room / fp4g::rows_stage_bytes(mx != 0, plan.tn);
   if (plan.stages > fp4g::ROWS_MAX_STAGES) plan.stages = fp4g::ROWS_MAX_STAGES;
   while (fp4g::rows_tmem_cols(mx != 0, plan.tn, plan.stages) > 512 / ctas) plan.stages--;
+  // the tile and the other CTAs' parts lie over the stages (true for every choice above)
+  if (plan.stages * fp4g::rows_stage_bytes(mx != 0, plan.tn) < (2 * plan.tn + 8) * 512) plan.split = 1;
   return plan;
 }
 
