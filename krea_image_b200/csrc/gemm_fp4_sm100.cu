@@ -339,7 +339,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     tc_fence_after();
   }
   __syncwarp();
-  if (split > 1) cluster_arrive();           // nothing uses this CTA's stages any more
+  if (split > 1) cluster_arrive_relaxed();   // nothing uses this CTA's stages any more
   if (warp >= 2) {
     const int quarter = warp & 3;
     if (done) {
@@ -373,26 +373,31 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     if (mine > 0) live = mbar_wait(received, 0, abort_word, SITE_PARTS) && live;
     __syncwarp();
-    cluster_arrive();                        // this CTA has what the others sent
+    cluster_arrive_relaxed();                // this CTA has what the others sent
   }
 
   // parts added in rank order, 8 columns of a row at a time
   const bool swiglu = p.epi == KREA_CUDA_EPI_SWIGLU;
   const int units_log2 = swiglu ? 3 : 4;
   const float alpha = scales.a * scales.w;
-  for (int u = threadIdx.x; live && u < mine << units_log2; u += ROWS_THREADS) {
+  const float *own = part + r0 * 128, *before = parts, *after = parts + (int)rank * share * 128;      // parts of CTAs below and above this one
+#pragma unroll 2
+  for (int u = threadIdx.x; u < (live ? mine << units_log2 : 0); u += ROWS_THREADS) {
     const int r = u >> units_log2, uc = u & ((1 << units_log2) - 1);
     const int c = swiglu ? (uc >> 2) * 64 + (uc & 3) * 8 : uc * 8;       // first of the tile's columns (SwiGLU: of the gate's)
     if (n0 + c >= p.N) continue;
     float f[8], g[8];
     const auto sum = [&](int col, float* o) {
+      const int at = r * 128 + col;
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] = 0.f;
-      for (uint32_t q = 0; q < split; q++) {
-        const float* from = q == rank ? part + (r0 + r) * 128 : parts + ((int)(q < rank ? q : q - 1) * share + r) * 128;
-        const float4 x = *(const float4*)(from + col), y = *(const float4*)(from + col + 4);
+      const auto add = [&](const float* from) {
+        const float4 x = *(const float4*)(from + at), y = *(const float4*)(from + at + 4);
         o[0] += x.x; o[1] += x.y; o[2] += x.z; o[3] += x.w; o[4] += y.x; o[5] += y.y; o[6] += y.z; o[7] += y.w;
-      }
+      };
+      for (uint32_t q = 0; q < rank; q++) add(before + q * share * 128);
+      add(own);
+      for (uint32_t q = rank + 1; q < split; q++) add(after + (q - rank - 1) * share * 128);
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] *= alpha;
     };
@@ -521,6 +526,8 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           tma_load_3d_pair(st + 2 * ROW_TILE_BYTES + C::S_BYTES, &tmWs, bar, 0, kb, n0 >> 7);
         }
       }
+      // the leader's products signal this CTA's barriers: the last ones are waited for here
+      for (uint32_t i = n > STAGES ? n - STAGES : 0; i < n && *abort_word == 0u; i++) mbar_wait(&empty[i % STAGES], (i / STAGES) & 1, abort_word, SITE_EMPTY);
       // nothing may still be in flight into this CTA's shared memory when it exits
       if (*abort_word != 0u && rank == 0) {
         for (uint32_t i = (n > STAGES ? n - STAGES : 0); i < n; i++) mbar_wait_slow(&full[i % STAGES], (i / STAGES) & 1, abort_word + 1, SITE_FULL);
@@ -586,11 +593,12 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster_relaxed(mapa(smem_u32(acc_empty), 0));
       const bool last = t + workers >= tiles;
-      if (last) {                  // this warp has no more business with the other CTA
-        cluster_arrive();
+      if (last) {                  // nobody waits for the accumulator any more, and this warp has no more business with the other CTA
+        cluster_arrive_relaxed();
         arrived = true;
+      } else if (lane == 0) {
+        mbar_arrive_cluster_relaxed(mapa(smem_u32(acc_empty), 0));
       }
       const int row0 = m0 + quarter * 32, col0 = n0 + half * 128;
       if (row0 >= p.M || col0 >= p.N) continue;
@@ -606,11 +614,11 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     if (lane == 0) tma_store_wait_read();      // the last box has left shared memory
     __syncwarp();
-    if (!arrived) cluster_arrive();
+    if (!arrived) cluster_arrive_relaxed();
   }
   if (warp < 4) {
     __syncwarp();
-    cluster_arrive();
+    cluster_arrive_relaxed();
   }
 
   // nobody leaves or frees tensor memory while the peer may still read this CTA's shared memory, signal its barriers or
