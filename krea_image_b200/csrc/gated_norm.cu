@@ -205,14 +205,14 @@ __global__ void __maxnreg__(REGS) gated_norm_kernel(const GatedNormParams p) {
       for (int k = 0; k < HOLD; k++) ss = fma8(v[k], v[k], ss);
       const F8 rr = splat(rsqrtf(cta_sum(total(ss), part[it][0]) * inv_w + p.eps));
 #pragma unroll
-      for (int k = 0; k < HOLD; k++) v[k] = mul8(v[k], mul8(rr, AHEAD ? w2[k] : vec(p.post, k, 1.f)));
+      for (int k = 0; k < HOLD; k++) v[k] = mul8(mul8(v[k], rr), AHEAD ? w2[k] : vec(p.post, k, 1.f));
     }
     F8 ss = splat(0.f);
 #pragma unroll
     for (int k = 0; k < HOLD; k++) {
       const int c = (t + k * blockDim.x) * 8;
       if (p.gate) v[k] = mul8(v[k], AHEAD ? w[k] : vec(gate, k, 1.f));
-      v[k] = fma8(xs, in.x[k], v[k]);
+      v[k] = add8(mul8(xs, in.x[k]), v[k]);          // each product rounded by itself, as the formula is written
       if (c < p.width && p.x_out) store8<V8>(p.x_out + (int64_t)row * p.ld_xo + c, v[k]);
       ss = fma8(v[k], v[k], ss);
     }
