@@ -14,8 +14,8 @@
 // are in x', so that they are under way through the sum, the norm and the stores; the arithmetic is on packed pairs.
 // HOLD = 2 up to 16384 columns, 4 above (whose 64 registers do not hold all of the row).  Fewer rows than two an SM take
 // HOLD = 1 and load the vectors a step before their use (AHEAD): there the time is one row's chain of accesses.
-// Measured at 4608 x 6144: bf16 56.6 us (93 % of the copy bandwidth), MX 55.9 us (83 %), NV 60.1 us (77 %); f32 with a
-// post-norm at 4748 x 2560 37.0 us (71 %); one row of 6144 3.4 us.  Vectors kept in shared memory instead of L1 measured
+// Measured at 4608 x 6144: bf16 57 us (92 % of the copy bandwidth), MX 55.5 us (83 %), NV 59.3 us (78 %); f32 with a
+// post-norm at 4748 x 2560 36.4 us (72 %); one row of 6144 3.4 us.  Vectors kept in shared memory instead of L1 measured
 // slower (NV 67.9 us, f32 43.6 us), as did one row a CTA without the loop (NV 75.7 us).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

@@ -9,8 +9,11 @@
 // Two kernels:
 //   gemm_fp4_rows_sm100   few rows of A: the 128 tensor-core rows are columns of C (rows of W), the rows of A (16 to 128)
 //                         are its columns, so the weights stream through once and no tensor-core row idles; the CTAs of a
-//                         cluster share K and add their parts through shared memory, in a fixed order.
-//   gemm_fp4_pair_sm100   many rows: 256 x 256 tiles on CTA pairs (cta_group::2), persistent, like the bf16 kernel.
+//                         cluster share K and add their parts through shared memory, in a fixed order.  HBM-bound:
+//                         1 x 15360 x 6144 NV 12 us, of which the 53 MB take 8.2 at the copy bandwidth.
+//   gemm_fp4_pair_sm100   many rows: 256 x 256 tiles on CTA pairs (cta_group::2), persistent, like the bf16 kernel.  A stage
+//                         moves 38 KB (NV) into each SM for 512 clocks of products, about what L2 delivers, and the clock falls to
+//                         1.5 GHz under the power cap: 4608 x 15360 x 6144 148-187 us (4.7-5.9 PFLOP/s) by the clock's state.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -671,18 +674,23 @@ static cudaError_t launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap
 Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force) {
   Fp4GemmPlan plan{};
   plan.split = 1;
-  plan.pair = force == 2 || (force == 0 && M > 128);
-  if (plan.pair) return plan;
-  // rows of A a CTA: all of them up to 128, in whole sixteens; above, tiles of 128 (a tile starts where its scales do)
+  // rows of A a CTA of the few-rows kernel: all of them up to 128, in whole sixteens; above, tiles of 128 (a tile starts where its
+  // scales do)
   const int shares = (M + 127) / 128;
   plan.tn = M < 128 ? (M + 15) & ~15 : 128;
   const int64_t tiles = (int64_t)((N + 127) / 128) * shares;
   const int kblocks = (K + fp4g::KB - 1) / fp4g::KB;
+  // Pairs above 128 rows, unless so few tiles would leave them idle through a long K that the few-rows kernel can share.  us, NV,
+  // few rows | pairs: 128 x 6144 x 6144 10.7 | 12.4, 256 x 6144 x 6144 14.2 | 12.7, 256 x 15360 x 6144 19.7 | 15.6; with tiles for
+  // half of the SMs: 512 x 2048 x 2048 8.2 | 7.2, 256 x 2504 x 2500 8.9 | 9.5, 512 x 2048 x 6144 10.9 | 11.9, 160 x 1024 x 16384 11.6 | 23.8
+  plan.pair = force == 2 || (force == 0 && M > 128 && !(tiles * 2 <= sms && kblocks >= 10));
+  if (plan.pair) return plan;
   // How K is shared: clusters of up to four CTAs (eight where a few tiles are all there is).  One CTA an SM with a deep ring
   // moves the most while clusters find room side by side: pairs on all SMs, larger ones on five in six (48 clusters of three
   // on 148 SMs ran in two rounds).  Where that leaves a quarter of the SMs idle and a CTA has at most 64 rows to finish, two
-  // CTAs an SM with short rings.  us, MX, K = 6144: 1 x 6144 deep 2 x 48 CTAs 7.7, short 4 x 48 6.1; 48 x 6144 8.5, 8.0;
-  // 77 x 6144 (K 16384) 16.1, 16.9; 128 x 6144 10.7, 12.3; 1 x 15360 deep 120 11.3, short 240 11.9; 64 x 8192 (K 2048) deep 1 x 64 7.0, 2 x 64 6.5.
+  // CTAs an SM with short rings.  us, MX: 64 x 6144 x 6144 deep 2 x 48 CTAs 9.0, deep 3 x 48 13.9, short 4 x 48 8.8;
+  // 64 x 2504 x 2500 deep 3 x 20 6.1, short 4 x 20 5.9; 96 x 6144 x 6144 deep 2 x 48 9.5; 1 x 15360 x 6144 deep 120 11.3, short
+  // 240 11.5; 64 x 8192 x 2048 deep 1 x 64 7.0, 2 x 64 6.3; 1 x 1024 x 8192 short 4 x 8 5.7, 8 x 8 4.5.
   const int top = tiles * 16 <= sms ? 8 : 4;
   const auto most = [&](auto room) {
     int c = 1;
