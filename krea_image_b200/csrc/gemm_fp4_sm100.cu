@@ -64,16 +64,19 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t saddr16) {
   else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 
-// Both tensor scales.  Asked for at the kernel's start and not where the compiler would put it, next to the use: a memory
-// latency at the end of every launch.  Multiplied at the use: before that nobody waits for them.
-struct TensorScales {
+// Both tensor scales, and whether an earlier kernel gave up on a wait (then nothing is stored).  Asked for at the kernel's start
+// and not where the compiler would put it, next to the use: a memory latency at the end of every launch.  Looked at only
+// at the use: before that nobody waits for them.
+struct Early {
   float a = 1.f, w = 1.f;
-  __device__ __forceinline__ explicit TensorScales(const Fp4GemmParams& p) {
+  uint32_t status = 0u;
+  __device__ __forceinline__ explicit Early(const Fp4GemmParams& p) {
     if (p.a_ts) asm volatile("ld.global.f32 %0, [%1];" : "=f"(a) : "l"(p.a_ts));
     if (p.w_ts) asm volatile("ld.global.f32 %0, [%1];" : "=f"(w) : "l"(p.w_ts));
+    if (p.status) asm volatile("ld.volatile.global.u32 %0, [%1];" : "=r"(status) : "l"(p.status));
   }
 };
-// An earlier kernel gave up on a wait: this one does nothing.  Looked at by a warp that has nothing else to do then.
+// The same for the loops, by a thread that has nothing else to do then: they stop early.
 __device__ __forceinline__ void check_status(const Fp4GemmParams& p, volatile uint32_t* abort_word) {
   if (p.status != nullptr && *(volatile uint32_t*)p.status != 0u) abort_word[0] = 0xFFu;
 }
@@ -275,7 +278,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   griddep_wait();
   griddep_launch();
   if (threadIdx.x == 64) check_status(p, abort_word);
-  const TensorScales scales(p);
+  const Early early(p);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -362,10 +365,10 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
   __syncwarp();
   __syncthreads();
-  bool live = *abort_word == 0u;
+  bool live = *abort_word == 0u && early.status == 0u;
   if (split > 1) {
     cluster_wait();
-    if (threadIdx.x == 0 && live) {
+    if (threadIdx.x == 0) {
       for (uint32_t q = 0; q < split; q++) {
         const int n = rows_of((int)q);
         if (q != rank && n > 0) {
@@ -374,7 +377,11 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
       }
     }
-    if (mine > 0) live = mbar_wait(received, 0, abort_word, SITE_PARTS) && live;
+    if (mine > 0 && !mbar_wait(received, 0, abort_word, SITE_PARTS)) {
+      live = false;
+      // what the others may have sent all the same has to land before this CTA says that it may leave
+      if (threadIdx.x == 0) mbar_wait_slow(received, 0, abort_word + 1, SITE_PARTS);
+    }
     __syncwarp();
     cluster_arrive_relaxed();                // this CTA has what the others sent
   }
@@ -382,7 +389,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   // parts added in rank order, 8 columns of a row at a time
   const bool swiglu = p.epi == KREA_CUDA_EPI_SWIGLU;
   const int units_log2 = swiglu ? 3 : 4;
-  const float alpha = scales.a * scales.w;
+  const float alpha = early.a * early.w;
   const float *own = part + r0 * 128, *before = parts, *after = parts + (int)rank * share * 128;      // parts of CTAs below and above this one
 #pragma unroll 2
   for (int u = threadIdx.x; u < (live ? mine << units_log2 : 0); u += ROWS_THREADS) {
@@ -582,8 +589,8 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     // with them: the tensor cores go on while the stores are under way.
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t src = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
-    const TensorScales scales(p);
-    const float alpha = scales.a * scales.w;
+    const Early early(p);
+    const float alpha = early.a * early.w;
     int it = 0;
     bool arrived = false;
     for (int t = worker; t < tiles; t += workers, it++) {
@@ -604,7 +611,7 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         mbar_arrive_cluster_relaxed(mapa(smem_u32(acc_empty), 0));
       }
       const int row0 = m0 + quarter * 32, col0 = n0 + half * 128;
-      if (row0 >= p.M || col0 >= p.N) continue;
+      if (row0 >= p.M || col0 >= p.N || __any_sync(0xffffffffu, early.status != 0u)) continue;
       if (p.epi == KREA_CUDA_EPI_RESID_GATE) {
         if (row0 + lane < p.M) pair_add(p, v, row0 + lane, col0, alpha);
       } else {

@@ -302,3 +302,52 @@ def test_calls_with_extreme_sizes_are_refused_before_any_launch(kc):
             call()
         assert e.value.code == B.E_ARG
     assert kc.launches == n0
+
+
+@pytest.mark.parametrize("tile", ["0", "1", "2"])
+def test_products_behind_a_wait_that_ran_out_store_nothing(monkeypatch, tile):
+    """An attention launch whose last K tile is never requested gives up after 5 ms; the products queued behind it must leave
+    their outputs as they were, and run again once the failure has been reported."""
+    monkeypatch.setenv("KREA_CUDA_FP4_TILE", tile)
+    k = ops.KreaCuda(0)
+    k.set_stream(torch.cuda.current_stream())
+    try:
+        H, T, gh, gw = 2, 128, 16, 24
+        S, ld = T + gh * gw, 3 * H * 128
+        rng = np.random.default_rng(78)
+        x = torch.from_numpy(synth.f32_to_bf16_bits(rng.standard_normal((S, ld)).astype(np.float32)).view(np.int16)).cuda().view(torch.bfloat16).view(-1)
+        one = torch.ones(128, device="cuda")
+        cos, sin = (torch.from_numpy(np.ascontiguousarray(t)).cuda() for t in synth.rope_tables_axial2d(T, gh, gw))
+        o = torch.zeros((S, H * 128), dtype=torch.bfloat16, device="cuda")
+        runs = []
+        for M, N, K, epi in ((1, 2048, 6144, B.EPI_BF16), (64, 128, 2100, B.EPI_SWIGLU), (17, 256, 300, B.EPI_RESID_GATE), (700, 1032, 2048, B.EPI_BF16), (300, 520, 200, B.EPI_RESID_GATE)):
+            a, w = (torch.from_numpy(rng.integers(0, 256, (r, ops.fp4_row_bytes(K)), dtype=np.uint8)).cuda() for r in (M, N))
+            sa, sw = (torch.full((ops.fp4_scale_bytes(B.FP4_NV, r, K),), 0x38, dtype=torch.uint8, device="cuda") for r in (M, N))
+            c = torch.full((M, N // 2 if epi == B.EPI_SWIGLU else N), 7.0, dtype=torch.float32 if epi == B.EPI_RESID_GATE else torch.bfloat16, device="cuda")
+            vec = torch.ones(N, device="cuda") if epi == B.EPI_RESID_GATE else None
+            runs.append((c, lambda a=a, sa=sa, w=w, sw=sw, c=c, M=M, N=N, K=K, epi=epi, vec=vec: k.gemm_fp4(a, sa, w, sw, c, M, N, K, a.shape[1], w.shape[1], c.shape[1], B.FP4_NV, epilogue=epi, vec=vec)))
+        for _, run in runs:
+            run()
+        k.wait()
+        want = [c.clone() for c, _ in runs]
+        assert all(not bool((w == 7.0).all()) for w in want)
+        for c, _ in runs:
+            c.fill_(7.0)
+        k.set_wait_limit(0.005)
+        k.test_drop_one_load(True)
+        k.joint_attention(x, x[H * 128:], x[2 * H * 128:], o, S, S, H, ld, ld, ld, H * 128, one, one, cos, sin)
+        k.test_drop_one_load(False)
+        for _, run in runs:
+            run()
+        with pytest.raises(ops.KreaCudaError) as e:
+            k.wait()
+        assert e.value.code == B.E_DEVICE
+        assert all(bool((c == 7.0).all()) for c, _ in runs)
+        k.set_wait_limit(2.0)
+        k.wait()
+        for (c, run), w in zip(runs, want):
+            run()
+            k.wait()
+            assert torch.equal(c, w)
+    finally:
+        k.close()
