@@ -14,9 +14,10 @@
 // are in x', so that they are under way through the sum, the norm and the stores; the arithmetic is on packed pairs.
 // HOLD = 2 up to 16384 columns, 4 above (whose 64 registers do not hold all of the row).  Fewer rows than two an SM take
 // HOLD = 1 and load the vectors a step before their use (AHEAD): there the time is one row's chain of accesses.
-// Measured at 4608 x 6144: bf16 57 us (92 % of the copy bandwidth), MX 55.5 us (83 %), NV 59.3 us (78 %); f32 with a
-// post-norm at 4748 x 2560 36.4 us (72 %); one row of 6144 3.4 us.  Vectors kept in shared memory instead of L1 measured
-// slower (NV 67.9 us, f32 43.6 us), as did one row a CTA without the loop (NV 75.7 us).
+// Measured at 4608 x 6144: bf16 56 us (93 % of the copy bandwidth), MX 51 us (90 %), NV 56 us (83 %); f32 with a
+// post-norm at 4748 x 2560 34 us (78 %); one row of 6144 3.4 us.  Measured slower: vectors kept in shared memory instead of
+// L1 (f32 43.6 us), one row a CTA without the loop (NV 75.7 us), rows brought by bulk copies into a ring in shared memory
+// (f32 35.0 us, NV 67 us: L1 is what the ring takes).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -304,6 +305,10 @@ cudaError_t launch_gated_norm(const GatedNormParams& p, int sms, bool pdl, cudaS
   // Not programmatic: CTAs that start on an SM as the kernel before leaves it keep that kernel's split of L1 and shared memory,
   // and after a GEMM the vectors have no L1 to stay in (norm + 4-bit product at 4608 x 6144: 154 us against 135)
   pdl = false;
+  // Many thin threads hide the chain of a row's sums better than half as many with two pieces each (2560 columns, f32, post-norm:
+  // 34 us against 37; 4608 x 6144 NV 55.4 against 59.5, MX 51 against 55.5), as long as two rows fit side by side:
+  // at 8192 columns, where one does, NV takes 63 us against 56
+  if (padded <= 6144) return v8 ? launch_rows<1, 40, false, true>(p, threads(1), sms, pdl, stream) : launch_rows<1, 40, false, false>(p, threads(1), sms, pdl, stream);
   if (padded <= 16384) return v8 ? launch_rows<2, 64, false, true>(p, threads(2), sms, pdl, stream) : launch_rows<2, 64, false, false>(p, threads(2), sms, pdl, stream);
   return launch_rows<4, 64, false, false>(p, threads(4), sms, pdl, stream);
 }
