@@ -66,7 +66,8 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t saddr16) {
 
 // Both tensor scales, and whether an earlier kernel gave up on a wait (then nothing is stored).  Asked for at the kernel's start
 // and not where the compiler would put it, next to the use: a memory latency at the end of every launch.  Looked at only
-// at the use: before that nobody waits for them.
+// at the use: before that nobody waits for them.  The status says only what is stored: loads and products run to their end
+// either way, since CTAs of a cluster that stopped after different stages would leave loads and signals under way to one another.
 struct Early {
   float a = 1.f, w = 1.f;
   uint32_t status = 0u;
@@ -76,10 +77,6 @@ struct Early {
     if (p.status) asm volatile("ld.volatile.global.u32 %0, [%1];" : "=r"(status) : "l"(p.status));
   }
 };
-// The same for the loops, by a thread that has nothing else to do then: they stop early.
-__device__ __forceinline__ void check_status(const Fp4GemmParams& p, volatile uint32_t* abort_word) {
-  if (p.status != nullptr && *(volatile uint32_t*)p.status != 0u) abort_word[0] = 0xFFu;
-}
 __device__ __forceinline__ float gelu_tanh(float x) { return 0.5f * x * (1.0f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x))); }
 
 // Everything after the sum for 8 columns of one row (SwiGLU apart), and their store
@@ -277,7 +274,6 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const uint32_t tmem_base = *tmem_slot, sf_base = tmem_base + (uint32_t)rows_acc_cols(TN);
   griddep_wait();
   griddep_launch();
-  if (threadIdx.x == 64) check_status(p, abort_word);
   const Early early(p);
 
   if (warp == 0) {
@@ -430,7 +426,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
   if (threadIdx.x == 0 && p.status != nullptr) {
     const uint32_t a = *abort_word;
-    if (a != 0u && a != 0xFFu) atomicCAS(p.status, 0u, a | ((blockIdx.x & 0xFFFu) << 8));
+    if (a != 0u) atomicCAS(p.status, 0u, a | ((blockIdx.x & 0xFFFu) << 8));
   }
 }
 
@@ -518,7 +514,6 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   tile_origin(worker, m0, n0);       // the divisions of the first tile are done before the wait
   griddep_wait();
   griddep_launch();
-  if (threadIdx.x == 96) check_status(p, abort_word);
   if (warp == 0) {
     if (lane == 0) {
       uint32_t n = 0;
@@ -643,7 +638,7 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
   if (threadIdx.x == 0 && p.status != nullptr) {
     const uint32_t a = *abort_word;
-    if (a != 0u && a != 0xFFu) atomicCAS(p.status, 0u, a | ((blockIdx.x & 0xFFFu) << 8));
+    if (a != 0u) atomicCAS(p.status, 0u, a | ((blockIdx.x & 0xFFFu) << 8));
   }
 }
 
