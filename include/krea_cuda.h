@@ -66,14 +66,14 @@ KREA_CUDA_API int krea_cuda_set_stream(krea_cuda* h, void* cuda_stream);
 KREA_CUDA_API int krea_cuda_sync(krea_cuda* h);
 /* Number of kernels this handle has launched so far. */
 KREA_CUDA_API uint64_t krea_cuda_launch_count(krea_cuda* h);
-/* Every wait inside the attention kernel (on a TMA load, a tensor-core product, another warp) gives up after
+/* Every wait inside the attention kernel and the 4-bit GEMM (on a TMA load, a tensor-core product, another warp) gives up after
  * this much device time, records where in a status word and lets the CTA run to its normal exit; krea_cuda_sync
  * then returns KREA_CUDA_E_DEVICE.  Default 2 s; accepted range 1 ms .. 60 s.  No counterpart in the reference
  * (Metal command buffers are bounded by the system's GPU watchdog instead). */
 KREA_CUDA_API int krea_cuda_set_wait_limit(krea_cuda* h, uint64_t nanoseconds);
 /* Test hook for that path: while on, the attention kernel's producer never requests the last K tile of a CTA,
- * so the wait for it runs out after the limit above.  Nothing faults and nothing waits longer than the limit;
- * the output of such a launch is meaningless.  Use with a limit of a few milliseconds. */
+ * and the 4-bit GEMM asks for less of its operands than it waits for, so the wait runs out after the limit
+ * above.  Nothing faults and nothing waits longer than a few times the limit; the output of such a launch is meaningless.  Use with a limit of a few milliseconds. */
 KREA_CUDA_API int krea_cuda_test_drop_one_load(krea_cuda* h, int on);
 /* Per-operator GPU timing, the counterpart of the reference's KREA_PROFILE marks (Metal::mark,
  * engine/src/metal.h:126-145): while enabled, every kernel launch is bracketed by CUDA events on the
@@ -406,7 +406,8 @@ KREA_CUDA_API int krea_cuda_fp4_dequantize(krea_cuda* h, const krea_cuda_fp4_deq
 /* C[M, N] = A x W^T on packed rows A [M, lda] and W [N, ldw] of one format, fp32 accumulation, times both tensor scales.
  * Epilogues and C as in krea_cuda_gemm: KREA_CUDA_EPI_BF16, _RESID_GATE, _SWIGLU, _F32, _GELU, _BIAS_BF16, _BIAS_F32
  * (_QKNORM_ROPE is KREA_CUDA_E_UNSUPPORTED: krea_cuda_joint_attention normalises and rotates Q and K itself).  Any M and K;
- * N and ldc multiples of 8, SwiGLU's N of 64.  The result depends on M, N and K only, not on what runs beside it. */
+ * N and ldc multiples of 8, SwiGLU's N of 64.  The result depends on M, N and K only, not on what runs beside it.
+ * A call that gave up on a wait (KREA_CUDA_E_DEVICE) leaves C unspecified: finished tiles are there, no unfinished one is. */
 typedef struct {
   const void* A;
   const void* a_scales;

@@ -91,6 +91,8 @@ struct Fp4GemmParams {
   uint32_t* status;
   int group_m;                  // set by the launcher, CTA pairs: row blocks per group of the tile order
   int tn, stages;               // set by the launcher, few rows: rows of A a CTA, stages of its ring
+  uint64_t wait_limit_ns;       // bound on every wait inside the kernel (device wall time)
+  int test_drop_load;           // test hook, few rows: the last stage of K is never requested, so that a bounded wait runs out
 };
 struct Fp4GemmPlan {
   bool pair;                    // 256 x 256 tiles on CTA pairs; else 128 weight columns x tn rows a CTA

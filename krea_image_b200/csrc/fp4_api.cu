@@ -102,7 +102,9 @@ int krea_cuda_gemm_fp4(krea_cuda* h, const krea_cuda_gemm_fp4_args* a) {
   CUtensorMap tmA, tmAs, tmW, tmWs, tmC;
   memset(&tmC, 0, sizeof(tmC));
   int rc;
-  if ((rc = make_values_map(h, &tmA, a->A, a->M, a->K, a->lda, plan.pair ? 128 : plan.tn, "A"))) return rc;
+  // test hook, CTA pairs: boxes that lack rows, so that the bytes that are waited for never all arrive
+  const int box_a = plan.pair ? (h->test_drop_last_k ? 64 : 128) : plan.tn;
+  if ((rc = make_values_map(h, &tmA, a->A, a->M, a->K, a->lda, box_a, "A"))) return rc;
   if ((rc = make_values_map(h, &tmW, a->W, a->N, a->K, a->ldw, 128, "W"))) return rc;
   if ((rc = make_scales_map(h, &tmAs, a->a_scales, a->format, a->M, a->K, 1, "a_scales"))) return rc;
   if ((rc = make_scales_map(h, &tmWs, a->w_scales, a->format, a->N, a->K, plan.pair ? 2 : 1, "w_scales"))) return rc;
@@ -113,6 +115,8 @@ int krea_cuda_gemm_fp4(krea_cuda* h, const krea_cuda_gemm_fp4_args* a) {
   p.vec = uses_vec ? a->vec : nullptr;
   p.a_ts = a->a_tensor_scale; p.w_ts = a->w_tensor_scale;
   p.status = h->status_dev;
+  p.wait_limit_ns = h->wait_limit_ns;
+  p.test_drop_load = h->test_drop_last_k;
   CUDA_TRY(h, launch_gemm_fp4(plan, tmA, tmAs, tmW, tmWs, tmC, p, sms(h), h->pdl, h->stream));
   h->launches++;
   return KREA_CUDA_OK;

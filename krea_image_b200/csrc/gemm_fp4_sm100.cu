@@ -242,7 +242,8 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   uint64_t* acc_full = empty + ROWS_MAX_STAGES;
   uint64_t* received = acc_full + 1;                     // the other CTAs' parts of this CTA's rows have arrived
   uint32_t* tmem_slot = (uint32_t*)(received + 1);
-  volatile uint32_t* abort_word = (volatile uint32_t*)(tmem_slot + 1);
+  volatile uint32_t* abort_word = (volatile uint32_t*)(tmem_slot + 1);      // [0] a wait ran out; [1], [2] the same, while what is under way is awaited
+  const uint64_t limit = p.wait_limit_ns;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t split = gridDim.z, rank = blockIdx.z;       // the cluster is the grid's z axis
@@ -261,7 +262,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     mbar_init(acc_full, 1);
     mbar_init(received, 1);
-    abort_word[0] = abort_word[1] = 0u;
+    abort_word[0] = abort_word[1] = abort_word[2] = 0u;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -280,8 +281,9 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (lane == 0) {
       int s = 0, done = 0;
       uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1 && *abort_word == 0u; kb++, done++) {
-        if (!mbar_wait(&empty[s], phase ^ 1u, abort_word, SITE_EMPTY)) break;
+      const int asked = kb1 - (p.test_drop_load && rank == split - 1 ? 1 : 0);
+      for (int kb = kb0; kb < asked && *abort_word == 0u; kb++, done++) {
+        if (!mbar_wait(&empty[s], phase ^ 1u, abort_word, SITE_EMPTY, limit)) break;
         uint8_t* st = smem + s * STAGE_BYTES;
         mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
         tma_load_3d(st, &tmW, &full[s], kb * 128, n0, 0);
@@ -292,7 +294,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       }
       // nothing may still be in flight into this CTA's shared memory when it exits
       if (*abort_word != 0u) {
-        for (int i = done > STAGES ? done - STAGES : 0; i < done; i++) mbar_wait_slow(&full[i % STAGES], (uint32_t)(i / STAGES) & 1u, abort_word + 1, SITE_FULL);
+        for (int i = done > STAGES ? done - STAGES : 0; i < done; i++) mbar_wait_slow(&full[i % STAGES], (uint32_t)(i / STAGES) & 1u, abort_word + 1, SITE_FULL, limit);
       }
     }
   } else if (warp == 1) {
@@ -300,10 +302,10 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     constexpr uint32_t HI = desc_hi(1024);
     const uint32_t ID = idesc(MX, 128, TN);
     const uint32_t smem16 = smem_u32(smem) >> 4;
-    int s = 0;
+    int s = 0, kb = kb0;
     uint32_t phase = 0;
-    for (int kb = kb0; kb < kb1; kb++) {
-      if (!mbar_wait(&full[s], phase, abort_word, SITE_FULL)) break;
+    for (; kb < kb1; kb++) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], phase, abort_word, SITE_FULL, limit))) break;      // the warp decides as one
       tc_fence_after();
       const uint32_t x = smem16 + s * (STAGE_BYTES >> 4), y = x + (ROW_TILE_BYTES >> 4), sx = y + (Y_BYTES >> 4), sy = sx + (S_BYTES >> 4);
       const uint32_t tx = sf_base + s * SF_COLS, ty = tx + 4 * PIECES;
@@ -323,7 +325,11 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       __syncwarp();
       if (++s == STAGES) s = 0, phase ^= 1u;
     }
-    if (leader) umma_commit(acc_full);
+    if (kb == kb1) {                         // a sum that lacks a part is never announced
+      if (leader) umma_commit(acc_full);
+    } else {                                 // products under way still read the stages
+      for (int i = max(0, kb - kb0 - STAGES); i < kb - kb0; i++) mbar_wait_slow(&empty[i % STAGES], (uint32_t)(i / STAGES) & 1u, abort_word + 2, SITE_EMPTY, limit);
+    }
     __syncwarp();
   }
   // Each CTA of the cluster finishes an equal share of the tile's rows.  The tile goes from tensor memory to this CTA's shared
@@ -337,7 +343,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   if (split > 1 && threadIdx.x == 0 && mine > 0) mbar_arrive_expect_tx(received, (split - 1) * (uint32_t)mine * 512u);
   bool done = true;
   if (warp >= 2) {
-    done = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_word, SITE_ACC_FULL));      // what follows takes whole warps
+    done = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_word, SITE_ACC_FULL, limit));      // what follows takes whole warps
     tc_fence_after();
   }
   __syncwarp();
@@ -361,10 +367,11 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
   __syncwarp();
   __syncthreads();
-  bool live = *abort_word == 0u && early.status == 0u;
+  const bool whole = *abort_word == 0u;
+  bool live = whole && early.status == 0u;
   if (split > 1) {
     cluster_wait();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && whole) {         // an incomplete part is not sent: those who need it give up on it and store nothing
       for (uint32_t q = 0; q < split; q++) {
         const int n = rows_of((int)q);
         if (q != rank && n > 0) {
@@ -373,10 +380,10 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
       }
     }
-    if (mine > 0 && !mbar_wait(received, 0, abort_word, SITE_PARTS)) {
+    if (mine > 0 && !mbar_wait(received, 0, abort_word, SITE_PARTS, limit)) {
       live = false;
       // what the others may have sent all the same has to land before this CTA says that it may leave
-      if (threadIdx.x == 0) mbar_wait_slow(received, 0, abort_word + 1, SITE_PARTS);
+      if (threadIdx.x == 0) mbar_wait_slow(received, 0, abort_word + 2, SITE_PARTS, limit);
     }
     __syncwarp();
     cluster_arrive_relaxed();                // this CTA has what the others sent
@@ -417,6 +424,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     finish8(p, f, m0 + r0 + r, col);
   }
+  if (!done) mbar_wait_slow(acc_full, 0, abort_word + 2, SITE_ACC_FULL, limit);      // products that are late may not meet a CTA that has left
   __syncwarp();
   __syncthreads();
   if (split > 1) cluster_wait();             // the others have what this CTA sent
@@ -467,7 +475,9 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   uint64_t* acc_full = empty + STAGES;                         // accumulator complete
   uint64_t* acc_empty = acc_full + 1;                          // accumulator in registers (the leader's, by both CTAs' epilogue warps)
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + 1);
+  // [0] a wait ran out; [1] the loading warp's; [2] the same, while what is under way is awaited
   volatile uint32_t* abort_word = (volatile uint32_t*)(tmem_slot + 1);
+  const uint64_t limit = p.wait_limit_ns;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();     // 0 = leader
@@ -487,7 +497,7 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 16);      // one arrival a warp: 512 threads' would take longer than the loads they report
-    abort_word[0] = abort_word[1] = 0u;
+    abort_word[0] = abort_word[1] = abort_word[2] = 0u;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -516,12 +526,18 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   griddep_launch();
   if (warp == 0) {
     if (lane == 0) {
+      // The two CTAs have to stop behind the same stage, or loads of one would be awaited by neither: so nothing but the
+      // stages' own barriers, which the products free in both, ends this loop, and its waits are longer than the two that the
+      // products' warp can spend between one stage and the next.
+      const uint64_t long_limit = 3 * limit;
       uint32_t n = 0;
-      for (int t = worker; t < tiles && *abort_word == 0u; t += workers) {
+      bool ok = true;
+      for (int t = worker; t < tiles && ok; t += workers) {
         if (t != worker) tile_origin(t, m0, n0);
         for (int kb = 0; kb < kblocks; kb++, n++) {
           const int s = n % STAGES;
-          if (!mbar_wait(&empty[s], ((n / STAGES) & 1) ^ 1, abort_word, SITE_EMPTY)) break;
+          ok = mbar_wait(&empty[s], ((n / STAGES) & 1) ^ 1, abort_word + 1, SITE_EMPTY, long_limit);
+          if (!ok) break;
           uint8_t* st = smem + s * STAGE_BYTES;
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE_BYTES);
           const uint32_t bar = mapa(smem_u32(&full[s]), 0);
@@ -532,10 +548,14 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
       }
       // the leader's products signal this CTA's barriers: the last ones are waited for here
-      for (uint32_t i = n > STAGES ? n - STAGES : 0; i < n && *abort_word == 0u; i++) mbar_wait(&empty[i % STAGES], (i / STAGES) & 1, abort_word, SITE_EMPTY);
-      // nothing may still be in flight into this CTA's shared memory when it exits
-      if (*abort_word != 0u && rank == 0) {
-        for (uint32_t i = (n > STAGES ? n - STAGES : 0); i < n; i++) mbar_wait_slow(&full[i % STAGES], (i / STAGES) & 1, abort_word + 1, SITE_FULL);
+      for (uint32_t i = n > STAGES ? n - STAGES : 0; i < n && ok; i++) ok = mbar_wait(&empty[i % STAGES], (i / STAGES) & 1, abort_word + 1, SITE_EMPTY, long_limit);
+      if (!ok) atomicCAS((uint32_t*)abort_word, 0u, SITE_EMPTY);
+      // nothing may still be in flight into either CTA's shared memory when it exits, loads (the leader's barriers count both
+      // CTAs') or the last tile's signal
+      if (*abort_word != 0u) {
+        if (!ok && rank == 0)
+          for (uint32_t i = (n > STAGES ? n - STAGES : 0); i < n; i++) mbar_wait_slow(&full[i % STAGES], (i / STAGES) & 1, abort_word + 2, SITE_FULL, limit);
+        mbar_wait_slow(acc_full, (uint32_t)((tiles - 1 - worker) / workers) & 1u, abort_word + 2, SITE_ACC_FULL, limit);
       }
     }
   } else if (warp == 1 && rank == 0) {
@@ -546,12 +566,13 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     int it = 0;
     for (int t = worker; t < tiles; t += workers, it++) {
       if (it >= 1) {
-        if (!mbar_wait(acc_empty, (it - 1) & 1, abort_word, SITE_ACC_EMPTY)) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(acc_empty, (it - 1) & 1, abort_word, SITE_ACC_EMPTY, limit))) break;      // the warp decides as one
         tc_fence_after();
       }
-      for (int kb = 0; kb < kblocks; kb++, n++) {
+      int kb = 0;
+      for (; kb < kblocks; kb++, n++) {
         const int s = n % STAGES;
-        if (!mbar_wait(&full[s], (n / STAGES) & 1, abort_word, SITE_FULL)) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (n / STAGES) & 1, abort_word, SITE_FULL, limit))) break;
         tc_fence_after();
         const uint32_t a = smem16 + s * (STAGE_BYTES >> 4), w = a + (ROW_TILE_BYTES >> 4), sa = w + (ROW_TILE_BYTES >> 4), sw = sa + (C::S_BYTES >> 4);
         const uint32_t ta = sf_base + s * C::SF_COLS, tw = ta + 4 * PIECES;
@@ -572,12 +593,12 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
         __syncwarp();
       }
+      if (kb < kblocks) break;               // a sum that lacks a part is never announced
       if (leader) {
         umma_commit2(mapa(smem_u32(acc_full), 0));
         umma_commit2(mapa(smem_u32(acc_full), 1));
       }
       __syncwarp();
-      if (*abort_word != 0u) break;
     }
   } else if (warp >= 4) {
     // A thread takes one row and 128 columns into registers and hands the accumulator back before it does anything else
@@ -590,7 +611,7 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     bool arrived = false;
     for (int t = worker; t < tiles; t += workers, it++) {
       if (t != worker) tile_origin(t, m0, n0);
-      if (!__all_sync(0xffffffffu, mbar_wait(acc_full, it & 1, abort_word, SITE_ACC_FULL))) break;      // what follows takes whole warps
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full, it & 1, abort_word, SITE_ACC_FULL, limit))) break;      // what follows takes whole warps
       tc_fence_after();
       uint32_t v[128];
 #pragma unroll

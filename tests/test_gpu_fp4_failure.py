@@ -107,3 +107,38 @@ def test_products_behind_a_failure_run_to_their_normal_end(kt, fmt):
             r.run(kt)
             kt.wait()
             assert torch.equal(r.c, w)
+
+
+# one tile, a cluster that shares K, rows beyond one CTA, many stages a pair, more tiles than workers
+OWN = [(1, 128, 256, B.EPI_F32), (1, 2048, 6144, B.EPI_BF16), (64, 512, 2100, B.EPI_SWIGLU), (17, 256, 3000, B.EPI_RESID_GATE), (300, 520, 9000, B.EPI_RESID_GATE), (2600, 4160, 2048, B.EPI_BF16),
+       (2600, 4160, 520, B.EPI_RESID_GATE)]
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("shape", OWN, ids=lambda s: "x".join(map(str, s[:3])))
+def test_a_product_whose_wait_runs_out_stores_no_unfinished_sum(kt, shape, fmt):
+    """Operands that are not requested as a whole (a host-set hook; nothing faults) make the wait for them run out after 5 ms: few
+    rows, the last stage of K, which one CTA of a cluster has; CTA pairs, rows of A in every stage.  The sum lacks a part:
+    neither that CTA nor those it shares K with may store it."""
+    r = Product(11, fmt, *shape)
+    r.run(kt)
+    kt.wait()
+    want = r.c.clone()
+    assert not r.untouched()
+    for _ in range(2):
+        r.reset()
+        torch.cuda.synchronize()
+        kt.set_wait_limit(0.005)
+        kt.test_drop_one_load(True)
+        t0 = time.perf_counter()
+        r.run(kt)
+        kt.test_drop_one_load(False)
+        with pytest.raises(ops.KreaCudaError) as e:
+            kt.wait()
+        assert time.perf_counter() - t0 < 1.0                # a few times the limit
+        assert e.value.code == B.E_DEVICE and "4-bit" in str(e.value)
+        assert r.untouched()
+        kt.set_wait_limit(2.0)
+        r.run(kt)
+        kt.wait()
+        assert torch.equal(r.c, want)
