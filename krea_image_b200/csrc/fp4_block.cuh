@@ -120,12 +120,16 @@ __device__ __forceinline__ uint32_t nv_encode8_borders(const uint32_t* w, const 
 // scale near the ends of the f32 range, takes the comparisons.
 struct NvTable {
   uint2 e[128];          // x: inv as bits - positive: the product, negative: with a Newton step, 0: the comparisons; y: top of c | top of c - 1 << 16
-  float ts, inv6;
+  float ts;
+  float pre, inv6;       // their product is 1 / (6 ts); pre, a power of two, brings ts to where that is an f32
 };
 __device__ __forceinline__ void nv_table_fill(NvTable& t, float ts, int c) {     // c: 0 .. 127, one thread each
   if (c == 0) {
     t.ts = ts;
-    t.inv6 = 1.f / (6.f * ts);
+    // 6 ts passes the largest f32 above 5.67e37, and 1 / (6 ts) below 4.9e-40; amax * pre leaves the range only where the
+    // quotient is far beyond the highest or the lowest code
+    t.pre = ts < 0x1p-100f ? 0x1p60f : ts > 0x1p100f ? 0x1p-8f : 1.f;
+    t.inv6 = 1.f / (6.f * (ts * t.pre));
   }
   // border between a value and the next, times 6: passed from on when its code is odd (a tie goes to the even one), above it else
   const auto top = [&](uint32_t k) -> uint32_t {
@@ -156,11 +160,11 @@ __device__ __forceinline__ void nv_table_fill(NvTable& t, float ts, int c) {    
   else if (plain && c > 0 && c < 0x7E && on && !up && !down) f = -inv;      // not at the top of the scale's range, where x / s has no bound of its own
   t.e[c] = make_uint2(__float_as_uint(f), (top((uint32_t)c) & 0xFFFFu) | (below << 16));
 }
-// scale code of a block; the product with inv6 gives a code that is at most one off
+// scale code of a block; the product with 1 / (6 ts) gives a code that is at most one off
 __device__ __forceinline__ uint32_t nv_scale_code(uint32_t amax16, const NvTable& t) {
   if (amax16 >= 0x7F80u) return FP4_NAN_NV;
   uint16_t pair;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(0.f), "f"(__uint_as_float(amax16 << 16) * t.inv6));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(0.f), "f"(__uint_as_float(amax16 << 16) * t.pre * t.inv6));
   const uint32_t c = min((uint32_t)pair & 0x7Fu, 0x7Eu), tops = t.e[c].y;
   if (amax16 > (tops & 0xFFFFu)) return c + 1;
   return c > 0u && amax16 <= (tops >> 16) ? c - 1 : c;

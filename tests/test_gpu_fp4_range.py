@@ -1,0 +1,53 @@
+"""The 4-bit operators at the ends of their documented ranges, against the float64 statement in oracle/fp4_np.py: tensor scales
+next to the smallest and the largest f32."""
+import numpy as np
+import pytest
+import torch
+
+from krea_image_b200 import binding as B, ops
+from oracle import fp4_np
+from tests.test_gpu_fp4 import _dev, _f64, _quantise
+from tests.test_gpu_gated_norm import _case, _run
+
+pytestmark = pytest.mark.gpu
+
+# 6 ts leaves the f32 range above 5.67e37, 1 / (6 ts) below 4.9e-40; 2^-149 is the smallest f32
+ENDS = [3.3e38, 1e38, 6e37, 5.7e37, 5.6e37, 2.0 ** 126, 1e37, 1e-37, 2.0 ** -128, 5.1e-40, 4.8e-40, 4e-40, 2.0 ** -131, 2.0 ** -140, 1e-44, 2.0 ** -149]
+
+
+@pytest.fixture(scope="module")
+def kc():
+    k = ops.KreaCuda(0)
+    k.set_stream(torch.cuda.current_stream())
+    yield k
+    k.close()
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("ts", ENDS)
+def test_quantise_with_tensor_scales_at_the_ends_of_f32(kc, ts, transposed):
+    """Blocks with every finite bf16 magnitude as their largest (0 among them), and smaller ones all over the grid beside it."""
+    mags = np.arange(0x7F80, dtype=np.int64)
+    block = np.maximum(mags[:, None] - 41 * np.arange(16)[None, :], 0).astype(np.uint16)
+    block[:, 1::2] |= 0x8000
+    bits = block.reshape(-1, 64)
+    t = float(np.float32(ts))
+    assert 0 < t < np.inf
+    want_q, want_s = fp4_np.quantise(_f64(bits), "nv", t)
+    q, s = _quantise(kc, bits, "nv", ts, transposed)
+    assert np.array_equal(s, fp4_np.lay_out_scales(want_s, "nv", 64))
+    assert np.array_equal(q, fp4_np.pack(want_q, 64))
+
+
+@pytest.mark.parametrize("ts,size", [(3.3e38, 2e37), (1e38, 3e37), (6e37, 1e37), (2.0 ** -131, 1e-37), (4e-40, 1e-37), (1e-44, 1e-38), (2.0 ** -149, 2.0 ** -140), (4e-40, 1.0), (1e38, 1.0)])
+@pytest.mark.parametrize("rows,width", [(3, 264), (700, 1000)])
+def test_norm_with_tensor_scales_at_the_ends_of_f32(kc, rows, width, ts, size):
+    x, y, w, g, mul, add = _case(rows + width, rows, width, 1, False, True, True)
+    mul = (mul.astype(np.float64) * size).astype(np.float32)
+    mul[:, 32:64] = 0                                        # blocks of zeros
+    _, q, s = _run(kc, x, y, w, g, mul, None, "nv", h_ts=ts)
+    _, h, _ = _run(kc, x, y, w, g, mul, None, "bf16")
+    assert np.isfinite(h).all()
+    want_q, want_s = fp4_np.quantise(h, "nv", float(np.float32(ts)))
+    assert np.array_equal(s, fp4_np.lay_out_scales(want_s, "nv", width))
+    assert np.array_equal(q, fp4_np.pack(want_q, width))
