@@ -259,6 +259,9 @@ __global__ void __maxnreg__(REGS) gated_norm_kernel(const GatedNormParams p) {
             nv_encode<4>(u, code, nv, &q);
           }
           if (c < ((p.width + 31) & ~31)) *(uint32_t*)((uint8_t*)p.h + (int64_t)now * p.ld_h + (c >> 1)) = q;
+          // Blocks past the width get 0, whatever the row's factor made of their zeros (NaN, where it is not finite).  In a block that
+          // the width ends in, such a factor leaves no value finite before the width either.
+          if (c >= p.width) code = 0u;
           if ((t & (MX ? 3 : 1)) == 0 && c < chunks * 256) p.h_scales[scale_offset<MX>(now, MX ? c >> 5 : c >> 4, chunks)] = (uint8_t)code;
         }
       }

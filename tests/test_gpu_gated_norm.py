@@ -213,3 +213,20 @@ def test_many_rows(kc, rows, width, samples, y_f32, post, out, pad):
         want_x, want_h = fp4_np.gated_norm(f(x[r:r + 1]), f(y[r:r + 1]), None if w is None else f(w), f(gate[a:a + 1]), f(mul[a:a + 1]), f(add[a:a + 1]), 0.5, EPS, 0)
         yr = y[r:r + 1] if w is None else y[r:r + 1] / np.sqrt((f(y[r:r + 1]) ** 2).mean(1, keepdims=True) + EPS) * w
         _check(XO[r:r + 1].cpu().numpy(), H[r:r + 1, :width].double().cpu().numpy(), want_x, want_h, 0.5 * x[r:r + 1], y[r:r + 1], mul[a:a + 1], add[a:a + 1], width, out, yr, gate[a:a + 1])
+
+@pytest.mark.parametrize("out", ["mx", "nv"])
+@pytest.mark.parametrize("rows,width,post", [(6, 8, True), (6, 264, False), (7, 520, True), (130, 1000, True), (700, 520, True), (700, 1000, False), (6, 4120, True), (700, 8200, True), (6, 8200, False), (6, 16392, True)])
+def test_scales_past_the_width_stay_zero_in_rows_that_are_not_finite(kc, rows, width, post, out):
+    """Rows with a NaN, with an infinity, and of zeros without an eps: the 4-bit rows are the quantised bf16 rows, and past the width
+    there is nothing but zeros."""
+    x, y, w, g, mul, add = _case(rows + width, rows, width, 1, False, post, True)
+    x[1, 3], x[2, 5], y[4, width - 1], y[5, 0] = np.nan, np.inf, np.nan, -np.inf
+    for eps in (EPS, 0.0):
+        if eps == 0:
+            x[3], y[3] = 0, 0
+        xo, q, s = _run(kc, x, y, w, g, mul, add, out, eps=eps)
+        xb, h, _ = _run(kc, x, y, w, g, mul, add, "bf16", eps=eps)
+        assert np.array_equal(xo, xb, equal_nan=True) and np.isnan(h).any()
+        want_q, want_s = fp4_np.quantise(h, out)
+        assert np.array_equal(s, fp4_np.lay_out_scales(want_s, out, width))
+        assert np.array_equal(q, fp4_np.pack(want_q, width))
