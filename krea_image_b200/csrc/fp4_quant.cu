@@ -23,10 +23,10 @@ constexpr int FQ_THREADS = 256;
 // 16 values from `src` (16-byte aligned; `wide`: 32), zero from index `left` on
 __device__ __forceinline__ void load16(const __nv_bfloat16* src, int left, bool wide, uint32_t* w) {
   if (left >= 16 && wide) {       // one access a lane and not two, 32 bytes apart, that cost L1 twice the passes
-    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(src));
   } else if (left >= 16) {
-    const uint4 a = __ldg((const uint4*)src), b = __ldg((const uint4*)src + 1);
+    const uint4 a = ld_global_16B(src), b = ld_global_16B(src + 8);
     w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
     w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
   } else {
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_quantize_rows_kernel(const Fp4
   griddep_wait();
   __shared__ NvTable nv;
   if constexpr (!MX) {
-    if (threadIdx.x < 128) nv_table_fill(nv, p.tensor_scale ? __ldg(p.tensor_scale) : 1.f, threadIdx.x);
+    if (threadIdx.x < 128) nv_table_fill(nv, p.tensor_scale ? ld_global_f1(p.tensor_scale) : 1.f, threadIdx.x);
     __syncthreads();
   }
   const bool wide = (((uintptr_t)p.src | (uintptr_t)(p.ld * 2)) & 31u) == 0;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp4_quantize_cols_kernel(const 
   }
   griddep_wait();
   if constexpr (!MX) {
-    if (threadIdx.x < 128) nv_table_fill(nv, p.tensor_scale ? __ldg(p.tensor_scale) : 1.f, threadIdx.x);
+    if (threadIdx.x < 128) nv_table_fill(nv, p.tensor_scale ? ld_global_f1(p.tensor_scale) : 1.f, threadIdx.x);
   }
   __syncthreads();
   const auto request = [&](int s) {                // the next tile not asked for yet, if there is one
@@ -245,11 +245,11 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_dequantize_kernel(const Fp4Deq
   const bool narrow = items <= 0xFFFFFFFFll;            // a 64-bit division costs as much as the rest
   const bool wide = (((uintptr_t)p.out | (uintptr_t)(p.ldo * 2)) & 31u) == 0;
   griddep_wait();
-  const float ts = MX || !p.tensor_scale ? 1.f : __ldg(p.tensor_scale);
+  const float ts = MX || !p.tensor_scale ? 1.f : ld_global_f1(p.tensor_scale);
   for (int64_t it = (int64_t)blockIdx.x * FQ_THREADS + threadIdx.x; it < items; it += step) {
     const int row = narrow ? (int)((uint32_t)it / (uint32_t)per_row) : (int)(it / per_row), k0 = (int)(it - (int64_t)row * per_row) * 16;
-    const uint2 q = __ldg((const uint2*)(p.q + (int64_t)row * p.ldq + (k0 >> 1)));
-    const uint32_t code = __ldg(p.scales + scale_offset<MX>(row, MX ? k0 >> 5 : k0 >> 4, chunks));
+    const uint2 q = ld_global_8B(p.q + (int64_t)row * p.ldq + (k0 >> 1));
+    const uint32_t code = ld_global_u8(p.scales + scale_offset<MX>(row, MX ? k0 >> 5 : k0 >> 4, chunks));
     float s;
     if constexpr (MX) s = code == FP4_NAN_MX ? __uint_as_float(0x7FC00000u) : code == 0u ? 0x1p-127f : __uint_as_float(code << 23);
     else s = (code & 0x7Fu) == FP4_NAN_NV ? __uint_as_float(0x7FC00000u) : e4m3_value(code & 0x7Fu);

@@ -84,10 +84,10 @@ template <bool V8>
 __device__ __forceinline__ F8 load8(const float* s) {
   F8 r;
   if constexpr (V8) {
-    asm volatile("ld.global.nc.v4.b64 {%0, %1, %2, %3}, [%4];" : "=l"(r.p[0]), "=l"(r.p[1]), "=l"(r.p[2]), "=l"(r.p[3]) : "l"(s));
+    asm volatile("ld.global.v4.b64 {%0, %1, %2, %3}, [%4];" : "=l"(r.p[0]), "=l"(r.p[1]), "=l"(r.p[2]), "=l"(r.p[3]) : "l"(s));
   } else {
-    asm volatile("ld.global.nc.v2.b64 {%0, %1}, [%2];" : "=l"(r.p[0]), "=l"(r.p[1]) : "l"(s));
-    asm volatile("ld.global.nc.v2.b64 {%0, %1}, [%2];" : "=l"(r.p[2]), "=l"(r.p[3]) : "l"(s + 4));
+    asm volatile("ld.global.v2.b64 {%0, %1}, [%2];" : "=l"(r.p[0]), "=l"(r.p[1]) : "l"(s));
+    asm volatile("ld.global.v2.b64 {%0, %1}, [%2];" : "=l"(r.p[2]), "=l"(r.p[3]) : "l"(s + 4));
   }
   return r;
 }
@@ -156,7 +156,7 @@ __global__ void __maxnreg__(REGS) gated_norm_kernel(const GatedNormParams p) {
   RowPieces<HOLD, Y32> in;
   in.template fetch<V8>(p, (int)min(row, (unsigned)p.rows - 1u));      // not under a condition: the compiler would move it into the loop, to where it is used
   if constexpr (OUT == KREA_CUDA_OUT_FP4_NV) {       // read after the sums' barriers; a CTA of one warp has none
-    for (int c = t; c < 128; c += blockDim.x) nv_table_fill(nv, p.h_ts ? __ldg(p.h_ts) : 1.f, c);
+    for (int c = t; c < 128; c += blockDim.x) nv_table_fill(nv, p.h_ts ? ld_global_f1(p.h_ts) : 1.f, c);
     if (blockDim.x == 32) __syncwarp();
   }
   const float inv_w = 1.0f / (float)p.width;

@@ -82,7 +82,7 @@ __device__ __forceinline__ float gelu_tanh(float x) { return 0.5f * x * (1.0f + 
 // Everything after the sum for 8 columns of one row (SwiGLU apart), and their store
 __device__ __forceinline__ void finish8(const Fp4GemmParams& p, float* f, int row, int col) {
   if (p.epi == KREA_CUDA_EPI_BIAS_BF16 || p.epi == KREA_CUDA_EPI_BIAS_F32) {
-    const float4 a = __ldg((const float4*)(p.vec + col)), b = __ldg((const float4*)(p.vec + col) + 1);
+    const float4 a = ld_global_f4(p.vec + col), b = ld_global_f4(p.vec + col + 4);
     f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
   } else if (p.epi == KREA_CUDA_EPI_GELU) {
 #pragma unroll
@@ -93,7 +93,7 @@ __device__ __forceinline__ void finish8(const Fp4GemmParams& p, float* f, int ro
     float4* o = (float4*)((float*)p.C + at);
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      const float4 gt = p.vec ? __ldg((const float4*)(p.vec + col) + e) : make_float4(1.f, 1.f, 1.f, 1.f);
+      const float4 gt = p.vec ? ld_global_f4(p.vec + col + 4 * e) : make_float4(1.f, 1.f, 1.f, 1.f);
       float4 x = o[e];
       x.x = fmaf(gt.x, f[4 * e], x.x); x.y = fmaf(gt.y, f[4 * e + 1], x.y); x.z = fmaf(gt.z, f[4 * e + 2], x.z); x.w = fmaf(gt.w, f[4 * e + 3], x.w);
       o[e] = x;
@@ -161,7 +161,7 @@ __device__ __forceinline__ void pair_store(const Fp4GemmParams& p, const CUtenso
       for (int q = 0; q < 8; q++) {
         const int c = c0 + q * 4;
         float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p.epi == KREA_CUDA_EPI_BIAS_F32 && col0 + c < p.N) b = __ldg((const float4*)(p.vec + col0 + c));
+        if (p.epi == KREA_CUDA_EPI_BIAS_F32 && col0 + c < p.N) b = ld_global_f4(p.vec + col0 + c);
         put(q, __float_as_uint(acc(c) + b.x), __float_as_uint(acc(c + 1) + b.y), __float_as_uint(acc(c + 2) + b.z), __float_as_uint(acc(c + 3) + b.w));
       }
       send(col0 + c0);
@@ -191,7 +191,7 @@ __device__ __forceinline__ void pair_store(const Fp4GemmParams& p, const CUtenso
   } else if (p.epi == KREA_CUDA_EPI_BIAS_BF16) {
     bf16_boxes([&](float* f, int col) {
       if (col < p.N) {
-        const float4 a = __ldg((const float4*)(p.vec + col)), b = __ldg((const float4*)(p.vec + col) + 1);
+        const float4 a = ld_global_f4(p.vec + col), b = ld_global_f4(p.vec + col + 4);
         f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
       }
     });

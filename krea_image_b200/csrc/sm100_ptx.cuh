@@ -292,6 +292,35 @@ __device__ __forceinline__ uint64_t exp2_emulated_x2(uint64_t x2) {
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Loads from memory that an earlier kernel of the stream may have written, for kernels with a programmatic launch: no read-only
+// path (ld.global.nc, __ldg), since that memory may still be written while this grid already runs, and volatile, so that they
+// stay behind griddep_wait().
+__device__ __forceinline__ float ld_global_f1(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float4 ld_global_f4(const float* p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_global_u8(const uint8_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_global_8B(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_global_16B(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // 32 bytes to global memory in one instruction (the address must be 32-byte aligned).  A thread that writes its own
 // row piece by piece fills whole 32-byte sectors this way: a 16-byte store leaves half a sector for the L2 to fetch
 // from memory first, and a few thousand such fills in flight per SM stall the stores for thousands of clocks.

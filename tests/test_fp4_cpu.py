@@ -153,3 +153,13 @@ def test_oracle_grid_ties_and_saturation():
 def test_oracle_e4m3_is_the_format():
     torch = pytest.importorskip("torch")
     assert np.array_equal(fp4_np.E4M3, torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy())
+
+
+def test_kernels_that_start_early_use_no_read_only_loads():
+    """A kernel with a programmatic launch runs while the one before it may still write what it will read: the read-only path
+    is not for such memory, and a compiler may move its loads above the wait for the predecessor."""
+    for name in ("fp4_quant.cu", "gemm_fp4_sm100.cu", "gated_norm.cu", "fp4_block.cuh"):
+        with open(os.path.join(ROOT, "krea_image_b200", "csrc", name)) as f:
+            code = "\n".join(line.split("//")[0] for line in f)
+        for word in ("__ldg", "global.nc", "__restrict__"):
+            assert word not in code, (name, word)
