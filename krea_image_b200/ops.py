@@ -47,22 +47,22 @@ def _addr(t) -> int:
 
 
 class _Call:
-    """An argument structure that a handle fills anew for each call of one operator: packed in one go, which takes a third
-    of the time of building a ctypes structure field by field (1.7 us for 22 fields) - on the order of a small kernel."""
+    """Packs the argument structure of one operator in one go, which takes a third of the time of building a ctypes structure
+    field by field (1.7 us for 22 fields) - on the order of a small kernel.  Each call has bytes of its own: ctypes gives
+    up the interpreter lock inside a call, and another thread's call may be packed meanwhile."""
     _CODES = {ctypes.c_void_p: "P", ctypes.c_int: "i", ctypes.c_float: "f"}
 
     def __init__(self, fn, cls):
-        self.fn = fn
-        self.buf = bytearray(ctypes.sizeof(cls))
-        self.ref = ctypes.byref(cls.from_buffer(self.buf))
-        self.pack = struct.Struct("@" + "".join(self._CODES[t] for _, t in cls._fields_)).pack_into
+        self.fn = fn                # takes the handle and the structure (the data of a bytes object, 16-byte aligned) as plain pointers
+        self.pack = struct.Struct("@" + "".join(self._CODES[t] for _, t in cls._fields_) + "0P").pack
+        assert len(self.pack(*[0] * len(cls._fields_))) == ctypes.sizeof(cls)
 
     def __call__(self, h, *values):
         try:
-            self.pack(self.buf, 0, *values)
+            args = self.pack(*values)
         except struct.error as e:          # a size beyond 32 bits, or no whole number
             raise KreaCudaError(B.E_ARG, f"argument out of range: {e}") from None
-        return self.fn(h, self.ref)
+        return self.fn(h, args)
 
 
 class KreaCuda:
@@ -78,7 +78,9 @@ class KreaCuda:
     def _call(self, name, cls):
         c = self._calls.get(name)
         if c is None:
-            c = self._calls[name] = _Call(getattr(self.lib, "krea_cuda_" + name), cls)
+            fn = self.lib["krea_cuda_" + name]      # a function object of its own, apart from the one that binding.py describes
+            fn.restype, fn.argtypes = ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]
+            c = self._calls[name] = _Call(fn, cls)
         return c
 
     def close(self):

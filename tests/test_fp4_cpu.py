@@ -3,6 +3,7 @@ so that no refusal needs a device), layout of the ctypes mirrors, and the oracle
 import ctypes
 import os
 import subprocess
+import threading
 
 import numpy as np
 import pytest
@@ -163,3 +164,27 @@ def test_kernels_that_start_early_use_no_read_only_loads():
             code = "\n".join(line.split("//")[0] for line in f)
         for word in ("__ldg", "global.nc", "__restrict__"):
             assert word not in code, (name, word)
+
+
+def test_two_threads_on_one_handle_pass_their_own_arguments():
+    """The interpreter lock is given up inside a call: another thread's call of the same operator may be prepared meanwhile."""
+    seen, inside, go = {}, threading.Barrier(2), threading.Event()
+
+    def fake(_, args):
+        a = ctypes.cast(args, ctypes.POINTER(B.Fp4DequantizeArgs)).contents
+        if threading.current_thread() is first:      # the arguments are read only after the second call has been prepared
+            inside.wait(10)
+            assert go.wait(10)
+        seen[threading.current_thread()] = [getattr(a, f[0]) for f in a._fields_]
+        return 0
+
+    fn = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p)(fake)
+    call = ops._Call(fn, B.Fp4DequantizeArgs)
+    mine, other = [256, 512, 768, 1024, 5, 70, 48, 72, 1], [4096, 8192, None, 16384, 7, 32, 16, 32, 0]
+    first = threading.Thread(target=lambda: call(None, *mine))
+    first.start()
+    inside.wait(10)
+    assert call(None, *[v or 0 for v in other]) == 0
+    go.set()
+    first.join(10)
+    assert seen[first] == mine and seen[threading.current_thread()] == other
