@@ -102,10 +102,10 @@ __device__ __noinline__ float scale_sums(uint32_t src, int cols, float a, float 
 }
 __device__ __forceinline__ float gelu_tanh(float x) { return 0.5f * x * (1.0f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x))); }
 
-// Everything after the sum for 8 columns of one row (SwiGLU apart), and their store
-__device__ __forceinline__ void finish8(const Fp4GemmParams& p, float* f, int row, int col) {
+// Everything after the sum for 8 columns of one row (SwiGLU apart), and their store.  vec: p.vec, from after_wait()
+__device__ __forceinline__ void finish8(const Fp4GemmParams& p, const float* vec, float* f, int row, int col) {
   if (p.epi == KREA_CUDA_EPI_BIAS_BF16 || p.epi == KREA_CUDA_EPI_BIAS_F32) {
-    const float4 a = ld_global_f4(p.vec + col), b = ld_global_f4(p.vec + col + 4);
+    const float4 a = ld_global_f4(vec + col), b = ld_global_f4(vec + col + 4);
     f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
   } else if (p.epi == KREA_CUDA_EPI_GELU) {
 #pragma unroll
@@ -116,7 +116,7 @@ __device__ __forceinline__ void finish8(const Fp4GemmParams& p, float* f, int ro
     float4* o = (float4*)((float*)p.C + at);
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      const float4 gt = p.vec ? ld_global_f4(p.vec + col + 4 * e) : make_float4(1.f, 1.f, 1.f, 1.f);
+      const float4 gt = vec ? ld_global_f4(vec + col + 4 * e) : make_float4(1.f, 1.f, 1.f, 1.f);
       float4 x = o[e];
       x.x = fmaf(gt.x, f[4 * e], x.x); x.y = fmaf(gt.y, f[4 * e + 1], x.y); x.z = fmaf(gt.z, f[4 * e + 2], x.z); x.w = fmaf(gt.w, f[4 * e + 3], x.w);
       o[e] = x;
@@ -134,7 +134,7 @@ __device__ __forceinline__ void finish8(const Fp4GemmParams& p, float* f, int ro
 // through shared memory as boxes of 32 rows x 128 bytes by TMA, which writes whole lines and stops at the last row and
 // column by itself.  Stored from registers, 32 bytes of 32 rows at a time, a tile took 5000 clocks and held up the loads of
 // the next one (3800 clocks a tile lost at 4608 x 15360 x 6144).  box: one box, used again and again, or `many` in a row.
-__device__ __forceinline__ void pair_store(const Fp4GemmParams& p, const CUtensorMap& tmC, const uint32_t* v, int row0, int col0, float alpha, uint8_t* box, bool many, int lane) {
+__device__ __forceinline__ void pair_store(const Fp4GemmParams& p, const float* vec, const CUtensorMap& tmC, const uint32_t* v, int row0, int col0, float alpha, uint8_t* box, bool many, int lane) {
   const bool swiglu = p.epi == KREA_CUDA_EPI_SWIGLU, f32 = p.epi == KREA_CUDA_EPI_F32 || p.epi == KREA_CUDA_EPI_BIAS_F32;
   uint32_t dst = smem_u32(box) + lane * 128;
   // 16 bytes at place q of the lane's row, swizzled as the tensor map has it
@@ -184,7 +184,7 @@ __device__ __forceinline__ void pair_store(const Fp4GemmParams& p, const CUtenso
       for (int q = 0; q < 8; q++) {
         const int c = c0 + q * 4;
         float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p.epi == KREA_CUDA_EPI_BIAS_F32 && col0 + c < p.N) b = ld_global_f4(p.vec + col0 + c);
+        if (p.epi == KREA_CUDA_EPI_BIAS_F32 && col0 + c < p.N) b = ld_global_f4(vec + col0 + c);
         put(q, __float_as_uint(acc(c) + b.x), __float_as_uint(acc(c + 1) + b.y), __float_as_uint(acc(c + 2) + b.z), __float_as_uint(acc(c + 3) + b.w));
       }
       send(col0 + c0);
@@ -214,7 +214,7 @@ __device__ __forceinline__ void pair_store(const Fp4GemmParams& p, const CUtenso
   } else if (p.epi == KREA_CUDA_EPI_BIAS_BF16) {
     bf16_boxes([&](float* f, int col) {
       if (col < p.N) {
-        const float4 a = ld_global_f4(p.vec + col), b = ld_global_f4(p.vec + col + 4);
+        const float4 a = ld_global_f4(vec + col), b = ld_global_f4(vec + col + 4);
         f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
       }
     });
@@ -225,15 +225,30 @@ __device__ __forceinline__ void pair_store(const Fp4GemmParams& p, const CUtenso
     });
   }
 }
-// C (f32) += vec * acc for 128 columns of a row
-__device__ __forceinline__ void pair_add(const Fp4GemmParams& p, const uint32_t* v, int row, int col0, float alpha) {
+// C (f32) += vec * acc for a warp's 32 rows, a lane each, and 128 columns.  The vector's piece waits in shared memory (`piece`, 512
+// bytes): a load of it from global memory stays behind every store to C before it (367 us at 4608 x 6144 x 16384, not 196).
+__device__ __forceinline__ void pair_add(const Fp4GemmParams& p, const float* vec, const uint32_t* v, int row0, int col0, float alpha, uint8_t* piece, int lane) {
+  const uint32_t gates = smem_u32(piece);
+  float4 g = make_float4(1.f, 1.f, 1.f, 1.f);
+  if (vec && col0 + 4 * lane < p.N) g = ld_global_f4(vec + col0 + 4 * lane);
+  __syncwarp();                                  // the last tile's piece has been read
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(gates + lane * 16), "f"(g.x), "f"(g.y), "f"(g.z), "f"(g.w) : "memory");
+  __syncwarp();
+  if (row0 + lane >= p.M) return;
+  float* row = (float*)p.C + (int64_t)(row0 + lane) * p.ldc + col0;
 #pragma unroll
   for (int c = 0; c < 128; c += 8) {
     if (col0 + c >= p.N) break;
-    float f[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) f[e] = __uint_as_float(v[c + e]) * alpha;
-    finish8(p, f, row, col0 + c);
+    for (int e = 0; e < 8; e += 4) {
+      float4 gt, x = *(const float4*)(row + c + e);
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(gt.x), "=f"(gt.y), "=f"(gt.z), "=f"(gt.w) : "r"(gates + (c + e) * 4));
+      x.x = fmaf(gt.x, __uint_as_float(v[c + e]) * alpha, x.x);
+      x.y = fmaf(gt.y, __uint_as_float(v[c + e + 1]) * alpha, x.y);
+      x.z = fmaf(gt.z, __uint_as_float(v[c + e + 2]) * alpha, x.z);
+      x.w = fmaf(gt.w, __uint_as_float(v[c + e + 3]) * alpha, x.w);
+      *(float4*)(row + c + e) = x;
+    }
   }
 }
 
@@ -299,6 +314,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   griddep_wait();
   griddep_launch();
   const Early early(p);
+  const float* vec = after_wait(p.vec);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -447,7 +463,7 @@ gemm_fp4_rows_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       for (int e = 0; e < 8; e++) f[e] = f[e] * sigmoid_approx(f[e]) * g[e];
       col = ((n0 + c) >> 6) * 32 + (uc & 3) * 8;
     }
-    finish8(p, f, m0 + r0 + r, col);
+    finish8(p, vec, f, m0 + r0 + r, col);
   }
   if (!done) mbar_wait_slow(acc_full, 0, abort_word + 2, SITE_ACC_FULL, limit);      // products that are late may not meet a CTA that has left
   __syncwarp();
@@ -631,6 +647,7 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t src = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
     const Early early(p);
+    const float* vec = after_wait(p.vec);
     float alpha = MX ? 1.f : early.a * early.w;
     const bool normal = is_normal(alpha);
     int it = 0;
@@ -656,13 +673,13 @@ gemm_fp4_pair_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       const int row0 = m0 + quarter * 32, col0 = n0 + half * 128;
       if (row0 >= p.M || col0 >= p.N || __any_sync(0xffffffffu, early.status != 0u)) continue;
       if (p.epi == KREA_CUDA_EPI_RESID_GATE) {
-        if (row0 + lane < p.M) pair_add(p, v, row0 + lane, col0, alpha);
+        pair_add(p, vec, v, row0, col0, alpha, out_smem + (warp - 4) * C::OUT_BYTES, lane);
       } else {
         // All pairs end their tiles at about the same time, and 64 KB from every SM at once hold up the loads of the next ones:
         // the warps take turns over the next tile's products (4608 x 15360 x 6144: 183 -> 177 us NV, 176 -> 170 us MX)
         if (!last) __nanosleep((uint32_t)((warp - 4) * kblocks * PACE_NS));
         // after a worker's last tile the stages are free: every box of a warp has a place of its own there
-        pair_store(p, tmC, v, row0, col0, alpha, last ? smem + (warp - 4) * 4 * C::OUT_BYTES : out_smem + (warp - 4) * C::OUT_BYTES, last, lane);
+        pair_store(p, vec, tmC, v, row0, col0, alpha, last ? smem + (warp - 4) * 4 * C::OUT_BYTES : out_smem + (warp - 4) * C::OUT_BYTES, last, lane);
       }
     }
     if (lane == 0) tma_store_wait_read();      // the last box has left shared memory

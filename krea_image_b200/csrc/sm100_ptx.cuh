@@ -300,11 +300,6 @@ __device__ __forceinline__ float ld_global_f1(const float* p) {
   asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
   return v;
 }
-__device__ __forceinline__ float4 ld_global_f4(const float* p) {
-  float4 v;
-  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
-  return v;
-}
 __device__ __forceinline__ uint32_t ld_global_u8(const uint8_t* p) {
   uint32_t v;
   asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p));
@@ -318,6 +313,18 @@ __device__ __forceinline__ uint2 ld_global_8B(const void* p) {
 __device__ __forceinline__ uint4 ld_global_16B(const void* p) {
   uint4 v;
   asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// The same for memory that this kernel does not write itself: free to move between other accesses, as one that reads a vector
+// among stores has to be, but not above after_wait(), from which its address comes.
+__device__ __forceinline__ const float* after_wait(const float* p) {
+  asm volatile("" : "+l"(p)::"memory");
+  return p;
+}
+__device__ __forceinline__ float4 ld_global_f4(const float* p) {
+  float4 v;
+  asm("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
   return v;
 }
 
