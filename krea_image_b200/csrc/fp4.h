@@ -12,7 +12,8 @@ namespace krea {
 
 // Launches with programmatic stream serialisation when `pdl`: the kernel may set itself up (barriers, tensor memory) while
 // the one before it in the stream drains.  Every kernel launched through here touches memory only after griddep_wait(),
-// in every CTA, and lets its own successor start after that.  cluster: CTAs along the grid's z axis (or x when cluster_x).
+// in every CTA.  The products let their own successor start after that, the gated norm at its last rows, the others when they
+// end.  cluster: CTAs along the grid's z axis (or x when cluster_x).
 template <class... P, class... A>
 inline cudaError_t launch_kernel(void (*kernel)(P...), dim3 grid, int block, size_t smem, cudaStream_t stream, bool pdl, int cluster, bool cluster_x, A... args) {
   cudaLaunchConfig_t cfg = {};
@@ -64,7 +65,7 @@ struct Fp4QuantParams {
   int mx;                       // 1: blocks of 32, e8m0 scales; 0: blocks of 16, e4m3 scales
   uint32_t* status;             // the transposed form reports a wait that ran out here
 };
-cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, bool pdl, cudaStream_t stream);
+cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, int sms, bool pdl, cudaStream_t stream);
 // transposed: tm describes src as [K, rows] in boxes of 128 k x 128 rows, no swizzle
 cudaError_t launch_fp4_quantize_cols(const CUtensorMap& tm, const Fp4QuantParams& p, int sms, bool pdl, cudaStream_t stream);
 
@@ -77,7 +78,7 @@ struct Fp4DequantParams {
   int64_t ldq, ldo;
   int mx;
 };
-cudaError_t launch_fp4_dequantize(const Fp4DequantParams& p, bool pdl, cudaStream_t stream);
+cudaError_t launch_fp4_dequantize(const Fp4DequantParams& p, int sms, bool pdl, cudaStream_t stream);
 
 struct Fp4GemmParams {
   void* C;

@@ -72,7 +72,7 @@ int krea_cuda_fp4_quantize(krea_cuda* h, const krea_cuda_fp4_quantize_args* a) {
     if (r != CUDA_SUCCESS) return fail(h, KREA_CUDA_E_CUDA, "fp4_quantize: cuTensorMapEncodeTiled failed with %d", (int)r);
     CUDA_TRY(h, launch_fp4_quantize_cols(tm, p, sms(h), h->pdl, h->stream));
   } else {
-    CUDA_TRY(h, launch_fp4_quantize(p, h->pdl, h->stream));
+    CUDA_TRY(h, launch_fp4_quantize(p, sms(h), h->pdl, h->stream));
   }
   h->launches++;
   return KREA_CUDA_OK;
@@ -86,7 +86,7 @@ int krea_cuda_fp4_dequantize(krea_cuda* h, const krea_cuda_fp4_dequantize_args* 
   p.q = (const uint8_t*)a->q; p.scales = (const uint8_t*)a->scales; p.tensor_scale = a->tensor_scale; p.out = (__nv_bfloat16*)a->out;
   p.rows = a->rows; p.K = a->K; p.ldq = a->ldq; p.ldo = a->ldo; p.mx = a->format == KREA_CUDA_FP4_MX;
   CUDA_TRY(h, cudaSetDevice(h->device));
-  CUDA_TRY(h, launch_fp4_dequantize(p, h->pdl, h->stream));
+  CUDA_TRY(h, launch_fp4_dequantize(p, sms(h), h->pdl, h->stream));
   h->launches++;
   return KREA_CUDA_OK;
 }

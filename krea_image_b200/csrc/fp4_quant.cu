@@ -221,12 +221,12 @@ static dim3 shape_grid(int64_t cols, int64_t row_items, int64_t most, Fp4Shape* 
   return dim3((unsigned)x, (unsigned)y);
 }
 
-cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, bool pdl, cudaStream_t stream) {
+cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, int sms, bool pdl, cudaStream_t stream) {
   if (p.rows <= 0 || p.K <= 0) return cudaSuccess;
   const int64_t tiles = (p.rows + 127) / 128, chunks = (p.K + 255) / 256;
   Fp4Shape z;
   // MX: two rounds of the CTAs that fit.  NV: one round, since each fills its table first (4608 x 16384: 39 us, 45 with MX's)
-  const dim3 grid = shape_grid(chunks * (p.mx ? 1 : 2), tiles * (p.mx ? 32 : 16), 148 * (p.mx ? 16 : 4), &z);
+  const dim3 grid = shape_grid(chunks * (p.mx ? 1 : 2), tiles * (p.mx ? 32 : 16), (int64_t)sms * (p.mx ? 16 : 4), &z);
   return launch_kernel(p.mx ? fp4_quantize_rows_kernel<true> : fp4_quantize_rows_kernel<false>, grid, FQ_THREADS, 0, stream, pdl, 1, false, p, z);
 }
 
@@ -275,11 +275,11 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_dequantize_kernel(const Fp4Deq
   }
 }
 
-cudaError_t launch_fp4_dequantize(const Fp4DequantParams& p, bool pdl, cudaStream_t stream) {
+cudaError_t launch_fp4_dequantize(const Fp4DequantParams& p, int sms, bool pdl, cudaStream_t stream) {
   if (p.rows <= 0 || p.K <= 0) return cudaSuccess;
   const int64_t items = (int64_t)p.rows * ((p.K + 15) / 16);
   int64_t blocks = (items + FQ_THREADS - 1) / FQ_THREADS;
-  if (blocks > 148 * 64) blocks = 148 * 64;
+  if (blocks > (int64_t)sms * 64) blocks = (int64_t)sms * 64;
   return launch_kernel(p.mx ? fp4_dequantize_kernel<true> : fp4_dequantize_kernel<false>, dim3((unsigned)blocks), FQ_THREADS, 0, stream, pdl, 1, false, p);
 }
 

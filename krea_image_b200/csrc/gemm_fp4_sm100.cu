@@ -261,6 +261,8 @@ __host__ __device__ constexpr int rows_tmem_cols(bool mx, int tn, int stages) {
   const int used = rows_acc_cols(tn) + stages * rows_sf_cols(mx);
   return used <= 128 ? 128 : used <= 256 ? 256 : 512;
 }
+// The tile and the other CTAs' parts lie over the stages, (2 tn + 8) * 512 bytes at most.  They fit in every plan that shares K: a stage
+// has tn * 128 bytes and 18 KB more, and there are six stages, or three and 64 rows at most (two CTAs an SM).
 constexpr int ROWS_MAX_STAGES = 8;
 constexpr int ROWS_THREADS = 192;   // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 }  // namespace fp4g
@@ -774,8 +776,6 @@ Fp4GemmPlan plan_gemm_fp4(int M, int N, int K, int mx, int sms, int force) {
   plan.stages = room / fp4g::rows_stage_bytes(mx != 0, plan.tn);
   if (plan.stages > fp4g::ROWS_MAX_STAGES) plan.stages = fp4g::ROWS_MAX_STAGES;
   while (fp4g::rows_tmem_cols(mx != 0, plan.tn, plan.stages) > 512 / ctas) plan.stages--;
-  // the tile and the other CTAs' parts lie over the stages (true for every choice above)
-  if (plan.stages * fp4g::rows_stage_bytes(mx != 0, plan.tn) < (2 * plan.tn + 8) * 512) plan.split = 1;
   return plan;
 }
 
