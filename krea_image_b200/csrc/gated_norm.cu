@@ -79,12 +79,18 @@ __device__ __forceinline__ F8 from_bf16(uint4 u) {
 }
 
 // 8 floats in one access where every row starts on 32 bytes (V8), in two else.  One access a thread makes a warp's a
-// whole kilobyte; two of 16 bytes, 32 apart, cost twice the passes through L1.
-template <bool V8>
+// whole kilobyte; two of 16 bytes, 32 apart, cost twice the passes through L1.  NC: by the read-only path, which is only for kernels
+// that start when their predecessor has ended (4748 x 2560 f32 with post-norm 33.8 us, 34.5 without).
+template <bool V8, bool NC>
 __device__ __forceinline__ F8 load8(const float* s) {
   F8 r;
-  if constexpr (V8) {
+  if constexpr (V8 && NC) {
+    asm volatile("ld.global.nc.v4.b64 {%0, %1, %2, %3}, [%4];" : "=l"(r.p[0]), "=l"(r.p[1]), "=l"(r.p[2]), "=l"(r.p[3]) : "l"(s));
+  } else if constexpr (V8) {
     asm volatile("ld.global.v4.b64 {%0, %1, %2, %3}, [%4];" : "=l"(r.p[0]), "=l"(r.p[1]), "=l"(r.p[2]), "=l"(r.p[3]) : "l"(s));
+  } else if constexpr (NC) {
+    asm volatile("ld.global.nc.v2.b64 {%0, %1}, [%2];" : "=l"(r.p[0]), "=l"(r.p[1]) : "l"(s));
+    asm volatile("ld.global.nc.v2.b64 {%0, %1}, [%2];" : "=l"(r.p[2]), "=l"(r.p[3]) : "l"(s + 4));
   } else {
     asm volatile("ld.global.v2.b64 {%0, %1}, [%2];" : "=l"(r.p[0]), "=l"(r.p[1]) : "l"(s));
     asm volatile("ld.global.v2.b64 {%0, %1}, [%2];" : "=l"(r.p[2]), "=l"(r.p[3]) : "l"(s + 4));
@@ -166,7 +172,7 @@ __global__ void __maxnreg__(REGS) gated_norm_kernel(const GatedNormParams p) {
   const auto vec = [&](const float* base, int k, float none) {
     const int c = (t + k * (int)blockDim.x) * 8;
     F8 r = splat(none);
-    if (base && c < p.width) r = load8<V8>(base + c);
+    if (base && c < p.width) r = load8<V8, !AHEAD>(base + c);
     return r;
   };
   const auto total = [](const F8& s) {
@@ -289,7 +295,9 @@ static cudaError_t launch_rows_as(const GatedNormParams& p, int block, int sms, 
   // 61); with fewer, setting up twice costs more than that (4748 x 2560: 46 us against 37)
   const int64_t slots = (int64_t)sms * resident, want = p.rows >= 12 * slots ? 2 * slots : slots;
   const int grid = (int)(p.rows < want ? p.rows : want);
-  return launch_kernel(k, dim3((unsigned)grid), block, 0, stream, pdl, 1, false, p);
+  // Programmatic only with few rows (AHEAD).  CTAs that start on an SM as the kernel before leaves it keep that kernel's split of L1
+  // and shared memory, and after a GEMM the vectors have no L1 to stay in (norm + 4-bit product at 4608 x 6144: 134 us against 116)
+  return launch_kernel(k, dim3((unsigned)grid), block, 0, stream, AHEAD && pdl, 1, false, p);
 }
 template <int HOLD, int REGS, bool AHEAD, bool V8>
 static cudaError_t launch_rows(const GatedNormParams& p, int block, int sms, bool pdl, cudaStream_t stream) {
@@ -305,9 +313,6 @@ cudaError_t launch_gated_norm(const GatedNormParams& p, int sms, bool pdl, cudaS
   const uintptr_t vec32 = (uintptr_t)p.post | (uintptr_t)p.gate | (uintptr_t)p.mul | (uintptr_t)p.add | (uintptr_t)(p.mod_rows > 0 ? p.mod_ld * 4 : 0);
   const bool v8 = ((rows32 | vec32) & 31u) == 0;
   if (p.rows < 2 * sms && padded <= 8192) return launch_rows<1, 64, true, false>(p, threads(1), sms, pdl, stream);
-  // Not programmatic: CTAs that start on an SM as the kernel before leaves it keep that kernel's split of L1 and shared memory,
-  // and after a GEMM the vectors have no L1 to stay in (norm + 4-bit product at 4608 x 6144: 154 us against 135)
-  pdl = false;
   // Many thin threads hide the chain of a row's sums better than half as many with two pieces each (2560 columns, f32, post-norm:
   // 34 us against 37; 4608 x 6144 NV 55.4 against 59.5, MX 51 against 55.5), as long as two rows fit side by side:
   // at 8192 columns, where one does, NV takes 63 us against 56
