@@ -432,7 +432,8 @@ KREA_CUDA_API int krea_cuda_gemm_fp4(krea_cuda* h, const krea_cuda_gemm_fp4_args
  * (then x' = x_scale * x); x_out f32 [rows, ld_xo], may be x itself, NULL = not stored; h per `out`: bf16, f32, or packed 4-bit
  * rows (ld_h in BYTES) with h_scales, quantised from the bf16 rounding of h; NULL = no second norm.  post f32 [width] (NULL =
  * no norm of y).  gate, mul, add: f32 vectors of width, row r uses the one at (r / mod_rows) * mod_ld (mod_rows 0: the one at 0),
- * so that every sample of a batch has its own; gate NULL = 1, add NULL = 0.  width a multiple of 8, 32768 at most. */
+ * so that every sample of a batch has its own; gate NULL = 1, add NULL = 0.  width a multiple of 8, 32768 at most.  The squares are
+ * added in f32: a row whose mean square passes the largest f32 (values from 1e19 on) has the factor 0. */
 #define KREA_CUDA_OUT_BF16 0
 #define KREA_CUDA_OUT_F32 1
 #define KREA_CUDA_OUT_FP4_MX 2

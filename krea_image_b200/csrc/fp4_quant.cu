@@ -6,8 +6,8 @@
 //
 // HBM-bound: 2 bytes read and 0.53 (MX) or 0.56 (NV) written per value.  A warp takes the four blocks that share a
 // 4-byte word of scales from rows 32 apart, which makes its scale bytes one contiguous piece (16 or 32 bytes) and its
-// reads whole 128-byte lines.  Measured at 4608 x 16384: MX 29.8 us (99 % of the copy bandwidth), NV 38.8 us (77 %: the
-// instructions of the scales), back to bf16 32.0 and 33.6 us (92 and 89 %).
+// reads whole 128-byte lines.  Measured at 4608 x 16384: MX 30 us (98 % of the copy bandwidth), NV 39.5 us (76 %: the
+// instructions of the scales), back to bf16 32.3 and 33.6 us (92 and 89 %).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -95,7 +95,8 @@ __global__ void __launch_bounds__(FQ_THREADS) fp4_quantize_rows_kernel(const Fp4
 // The same for an input-major source [K, ld] (row k holds value k of every output row).  CTAs stay and walk over tiles of 128 k x
 // 128 rows, which TMA brings into a ring of three (zeros past K and past the last row); a lane has two neighbouring
 // output rows and a warp 32 k.  Packed rows and scales are collected in shared memory and leave as whole pieces.
-// Measured at 6144 x 15360, NV: 51 us (110 with a tile a CTA and loads through registers).
+// Measured at 6144 x 15360: NV 54 us (69 % of the copy bandwidth; twice that with a tile a CTA and loads through registers), MX 45 us
+// (83 %).
 constexpr int FT_K = 128, FT_N = 128, FT_THREADS = 256, FT_STAGES = 3, FT_TILE = FT_K * FT_N * 2;
 constexpr int FT_PACKED = FT_K / 2 + 16;             // a packed row's bytes and the step to the next in shared memory
 constexpr int FT_SMEM = FT_STAGES * FT_TILE + FT_N * FT_PACKED + FT_N * (FT_K / 16) + 64 + 128;

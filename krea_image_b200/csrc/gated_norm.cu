@@ -12,10 +12,11 @@
 // What counts is how much is under way at once, and how few instructions a value takes.  CTAs stay for many rows, one row
 // each at a time: a thread has HOLD pieces of 8 columns and asks for its pieces of the next row as soon as those of this one
 // are in x', so that they are under way through the sum, the norm and the stores; the arithmetic is on packed pairs.
-// HOLD = 2 up to 16384 columns, 4 above (whose 64 registers do not hold all of the row).  Fewer rows than two an SM take
-// HOLD = 1 and load the vectors a step before their use (AHEAD): there the time is one row's chain of accesses.
-// Measured at 4608 x 6144: bf16 56 us (93 % of the copy bandwidth), MX 51 us (90 %), NV 56 us (83 %); f32 with a
-// post-norm at 4748 x 2560 34 us (78 %); one row of 6144 3.4 us.  Measured slower: vectors kept in shared memory instead of
+// HOLD = 1 with 40 registers up to 6144 columns, 2 up to 16384, 4 above (whose 64 registers do not hold all of the row: it spills).
+// Fewer rows than two an SM, of 8192 columns at most, take HOLD = 1 with 64 registers and load the vectors a step before their use
+// (AHEAD): there the time is one row's chain of accesses.
+// Measured at 4608 x 6144: bf16 57 us (93 % of the copy bandwidth), MX 52 us (88 %), NV 58 us (80 %); f32 with a
+// post-norm at 4748 x 2560 31-34 us (78-85 %); one row of 6144 3.4 us; 4608 x 20480 bf16 376 us (47 %), NV 425 us (36 %).  Measured slower: vectors kept in shared memory instead of
 // L1 (f32 43.6 us), one row a CTA without the loop (NV 75.7 us), rows brought by bulk copies into a ring in shared memory
 // (f32 35.0 us, NV 67 us: L1 is what the ring takes).
 #include <cuda_bf16.h>
@@ -291,8 +292,8 @@ static cudaError_t launch_rows_as(const GatedNormParams& p, int block, int sms, 
   // CTAs an SM holds: each of its four parts has 512 registers for a lane
   int resident = 4 * (512 / REGS) / (block / 32);
   resident = resident < 1 ? 1 : resident > 32 ? 32 : resident;
-  // with a dozen rows or more for each of them, two rounds of CTAs: the second evens out the ends (4608 x 6144: 56 us against
-  // 61); with fewer, setting up twice costs more than that (4748 x 2560: 46 us against 37)
+  // with a dozen rows or more for each of them, two rounds of CTAs: the second evens out the ends (4608 x 6144 bf16: 57 us
+  // against 63); with fewer, setting up twice costs more than that (4748 x 2560: 37 us against 35)
   const int64_t slots = (int64_t)sms * resident, want = p.rows >= 12 * slots ? 2 * slots : slots;
   const int grid = (int)(p.rows < want ? p.rows : want);
   // Programmatic only with few rows (AHEAD).  CTAs that start on an SM as the kernel before leaves it keep that kernel's split of L1

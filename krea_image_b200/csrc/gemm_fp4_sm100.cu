@@ -12,8 +12,9 @@
 //                         cluster share K and add their parts through shared memory, in a fixed order.  HBM-bound:
 //                         1 x 15360 x 6144 NV 12 us, of which the 53 MB take 8.2 at the copy bandwidth.
 //   gemm_fp4_pair_sm100   many rows: 256 x 256 tiles on CTA pairs (cta_group::2), persistent, like the bf16 kernel.  A stage
-//                         moves 38 KB (NV) into each SM for 512 clocks of products, about what L2 delivers, and the clock falls to
-//                         1.5 GHz under the power cap: 4608 x 15360 x 6144 148-187 us (4.7-5.9 PFLOP/s) by the clock's state.
+//                         moves 38 KB (NV) into each SM for 512 clocks of products, about what L2 delivers, and the clock falls under the
+//                         power cap, to 1.55 GHz in a short run and 1.35 in a long one: 4608 x 15360 x 6144 NV 184 us in a run of two
+//                         seconds (4.7 PFLOP/s), 156 us among single launches.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
