@@ -68,8 +68,9 @@ KREA_CUDA_API int krea_cuda_sync(krea_cuda* h);
 KREA_CUDA_API uint64_t krea_cuda_launch_count(krea_cuda* h);
 /* Every wait inside the attention kernel and the 4-bit GEMM (on a TMA load, a tensor-core product, another warp) gives up after
  * this much device time, records where in a status word and lets the CTA run to its normal exit; krea_cuda_sync
- * then returns KREA_CUDA_E_DEVICE.  Default 2 s; accepted range 1 ms .. 60 s.  No counterpart in the reference
- * (Metal command buffers are bounded by the system's GPU watchdog instead). */
+ * then returns KREA_CUDA_E_DEVICE.  Default 2 s; accepted range 1 ms .. 60 s.  One wait of the 4-bit GEMM
+ * lasts as long as a whole tile's K (some 0.35 us for each 256 values), so a short limit also bounds the K that can be summed.  No
+ * counterpart in the reference (Metal command buffers are bounded by the system's GPU watchdog instead). */
 KREA_CUDA_API int krea_cuda_set_wait_limit(krea_cuda* h, uint64_t nanoseconds);
 /* Test hook for that path: while on, the attention kernel's producer never requests the last K tile of a CTA,
  * and the 4-bit GEMM asks for less of its operands than it waits for, so the wait runs out after the limit

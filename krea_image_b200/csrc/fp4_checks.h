@@ -18,7 +18,7 @@ inline int64_t fp4_scale_tile_bytes(int format) { return format == KREA_CUDA_FP4
 inline int64_t fp4_scale_bytes(int format, int64_t rows, int64_t K) { return (rows + 127) / 128 * ((K + 255) / 256) * fp4_scale_tile_bytes(format); }
 
 // sizes beyond these are refused: rounding them up to whole tiles stays within 32 bits, and the product's longest wait
-// (for a whole tile's K) far below the limit of two seconds on every wait
+// (for a whole tile's K) far below the usual limit of two seconds on every wait
 constexpr int FP4_MAX_ROWS = 1 << 30, FP4_MAX_K = 1 << 26;
 
 inline bool off16(const void* p) { return ((uintptr_t)p & 15u) != 0; }

@@ -69,14 +69,14 @@ PAIRS = [(1e-30, 1e-14), (1e-14, 1e-30), (2.0 ** -70, 2.0 ** -70), (3e-39, 1e-4)
 
 
 @pytest.mark.parametrize("a_ts,w_ts", PAIRS)
-@pytest.mark.parametrize("M,N,K", [(1, 128, 512), (40, 264, 512), (300, 520, 512)])
+@pytest.mark.parametrize("M,N,K", [(1, 128, 512), (40, 264, 512), (300, 520, 512), (2600, 4160, 200)])      # the last: more tiles than CTA pairs
 def test_product_with_tensor_scales_whose_product_leaves_f32(kt, M, N, K, a_ts, w_ts):
     """Every block scale is 448: sums are multiples of 224^2 and below 2^24 of them, so that f32 holds them exactly, and what is
     left are two roundings, by 2^-24 or half of the smallest f32 each.  Sums of zero stay zero."""
     rng = np.random.default_rng(M + N)
     qa, qw = rng.integers(0, 16, (M, K)).astype(np.uint8), rng.integers(0, 16, (N, K)).astype(np.uint8)
     qw[::5] = 0
-    sc = [np.full((r, K // 16), 0x7E, np.uint8) for r in (M, N)]
+    sc = [np.full((r, -(-K // 16)), 0x7E, np.uint8) for r in (M, N)]
     (A, As, va), (W, Ws, vw) = (_operand(q, c, "nv", K) for q, c in zip((qa, qw), sc))
     a, w = float(np.float32(a_ts)), float(np.float32(w_ts))
     acc = va @ vw.T
