@@ -31,6 +31,19 @@ inline bool overlap(const void* a, int64_t n, const void* b, int64_t m) {
 // bytes that a matrix of `rows` rows of `width` used bytes, `ld` bytes apart, spans
 inline int64_t span(int64_t rows, int64_t width, int64_t ld) { return rows > 0 ? (rows - 1) * ld + width : 0; }
 
+// whether two matrices of rows (bytes used of a row, bytes between rows) have a byte in common; rows the same distance apart may
+// lie side by side in one buffer
+struct Rows {
+  const void* p;
+  int64_t rows, width, ld;
+};
+inline bool overlap(const Rows& a, const Rows& b) {
+  if (!overlap(a.p, span(a.rows, a.width, a.ld), b.p, span(b.rows, b.width, b.ld))) return false;
+  if (a.ld != b.ld) return true;
+  const int64_t from = ((intptr_t)b.p - (intptr_t)a.p) % a.ld, at = from < 0 ? from + a.ld : from;      // where b's rows start in a's
+  return at < a.width || at + b.width > a.ld;
+}
+
 inline const char* check_fp4_quantize(const krea_cuda_fp4_quantize_args* a) {
   if (a->rows < 0 || a->K < 0) return "negative size";
   if (a->rows > FP4_MAX_ROWS || a->K > FP4_MAX_K) return "rows must be 2^30 at most, K 2^26";
@@ -129,12 +142,13 @@ inline const char* check_gated_norm(const krea_cuda_gated_norm_args* a) {
   if (a->mod_rows < 0) return "mod_rows must not be negative";
   if (a->mod_rows > 0 && (a->mod_ld % 4 || a->mod_ld < 0)) return "mod_ld must be a multiple of 4, not negative";
   if (!(a->eps >= 0.f) || !isfinite(a->x_scale)) return "eps must not be negative, x_scale finite";
-  const int64_t xb = span(R, W * 4, (int64_t)a->ld_x * 4), xob = a->x_out ? span(R, W * 4, (int64_t)a->ld_xo * 4) : 0;
-  const int64_t yb = a->y ? span(R, W * (a->y_f32 ? 4 : 2), (int64_t)a->ld_y * (a->y_f32 ? 4 : 2)) : 0;
+  const int64_t es = a->y_f32 ? 4 : 2;
+  const Rows x = {a->x, R, W * 4, (int64_t)a->ld_x * 4}, y = {a->y, R, W * es, (int64_t)a->ld_y * es}, xo = {a->x_out, R, W * 4, (int64_t)a->ld_xo * 4}, h = {a->h, R, hb, hld};
+  const int64_t xb = span(R, x.width, x.ld), xob = a->x_out ? span(R, xo.width, xo.ld) : 0, yb = a->y ? span(R, y.width, y.ld) : 0;
   const int64_t hs = a->h ? span(R, hb, hld) : 0, sb = a->h && q ? fp4_scale_bytes(fmt, R, W) : 0;
-  if (a->x_out && overlap(a->x_out, xob, a->x, xb) && !((const void*)a->x_out == (const void*)a->x && a->ld_xo == a->ld_x)) return "x_out may be x itself with the same ld, or apart from it";
-  if (overlap(a->x_out, xob, a->y, yb)) return "x_out overlaps y";
-  if (overlap(a->h, hs, a->x, xb) || overlap(a->h, hs, a->y, yb) || overlap(a->h, hs, a->x_out, xob)) return "h overlaps another tensor";
+  if (overlap(xo, x) && !((const void*)a->x_out == (const void*)a->x && a->ld_xo == a->ld_x)) return "x_out may be x itself with the same ld, or apart from it";
+  if (overlap(xo, y)) return "x_out overlaps y";
+  if (overlap(h, x) || overlap(h, y) || overlap(h, xo)) return "h overlaps another tensor";
   if (overlap(a->h_scales, sb, a->x, xb) || overlap(a->h_scales, sb, a->y, yb) || overlap(a->h_scales, sb, a->x_out, xob) || overlap(a->h_scales, sb, a->h, hs))
     return "h_scales overlaps another tensor";
   const int64_t vb = (a->mod_rows > 0 ? (R - 1) / a->mod_rows * a->mod_ld : 0) * 4 + W * 4;      // from the first vector to the end of the last

@@ -194,3 +194,18 @@ def test_two_threads_on_one_handle_pass_their_own_arguments():
     go.set()
     first.join(10)
     assert seen[first] == mine and seen[threading.current_thread()] == other
+
+
+def test_gated_norm_takes_rows_side_by_side_in_one_buffer(checks):
+    """Column slices of one wide buffer have no byte in common; slices that do, and rows of another distance, are refused."""
+    base = dict(x=P[0], y=P[1], x_out=P[2], h=P[3], mul=P[8], rows=5, width=40, ld_x=128, ld_y=256, ld_xo=128, ld_h=256, mod_rows=0, mod_ld=0, x_scale=1.0, eps=1e-6, y_f32=0, out=B.OUT_BF16)
+    ok = lambda **ch: checks.gated_norm(ctypes.byref(B.GatedNormArgs(**{**base, **ch}))) is None  # noqa: E731
+    assert ok()
+    assert ok(h=P[1] + 80) and ok(h=P[1] + 256) and ok(y=P[3] + 80)             # y and h: 80 bytes of every 512
+    assert ok(x_out=P[0] + 160) and ok(x_out=P[0] + 352) and ok(x=P[2] + 160)    # x and x_out: 160 bytes of every 512
+    assert ok(x_out=P[1] + 80) and ok(h=P[2] + 160) and ok(h=P[0] + 160)
+    assert ok(h=P[1] + 512 - 80) and ok(h=P[1] - 80) and ok(h=P[1] + 3 * 512 + 80)
+    assert not ok(h=P[1] + 64) and not ok(h=P[1] + 512 - 64) and not ok(h=P[1] - 64) and not ok(h=P[1] + 4 * 512)
+    assert not ok(x_out=P[0] + 144) and not ok(x_out=P[0] + 368) and not ok(x_out=P[0] + 512)
+    assert not ok(h=P[1] + 80, ld_h=248) and not ok(x_out=P[0] + 160, ld_xo=124)
+    assert not ok(h=P[1] + 80, ld_h=512, out=B.OUT_FP4_MX, h_scales=P[1] + 160)

@@ -230,3 +230,24 @@ def test_scales_past_the_width_stay_zero_in_rows_that_are_not_finite(kc, rows, w
         want_q, want_s = fp4_np.quantise(h, out)
         assert np.array_equal(s, fp4_np.lay_out_scales(want_s, out, width))
         assert np.array_equal(q, fp4_np.pack(want_q, width))
+
+
+@pytest.mark.parametrize("rows,width", [(3, 40), (130, 1000), (700, 2568), (400, 8200)])
+def test_rows_side_by_side_in_one_buffer(kc, rows, width):
+    """x beside x_out and y beside h, each pair as column slices of one buffer: the same bits as apart, nothing else written."""
+    g = torch.Generator("cuda").manual_seed(rows)
+    x, y = torch.randn(rows, width, device="cuda", generator=g), torch.randn(rows, width, device="cuda", generator=g).bfloat16()
+    gate, mul, add = (torch.randn(width, device="cuda", generator=g) for _ in range(3))
+    xo, h = torch.empty_like(x), torch.empty_like(y)
+    kc.gated_norm(x, y, xo, h, rows, width, width, width, width, width, gate=gate, mul=mul, add=add)
+    ld = 2 * width + 24
+    a, b = torch.full((rows, ld), 9.0, device="cuda"), torch.full((rows, ld), 9.0, dtype=torch.bfloat16, device="cuda")
+    for first in (0, width + 8):                           # the input before the output, and behind it
+        second = width + 8 - first
+        a.fill_(9.0), b.fill_(9.0)
+        a[:, first:first + width], b[:, first:first + width] = x, y
+        kc.gated_norm(a[:, first:], b[:, first:], a[:, second:], b[:, second:], rows, width, ld, ld, ld, ld, gate=gate, mul=mul, add=add)
+        kc.wait()
+        assert torch.equal(a[:, second:second + width], xo) and torch.equal(b[:, second:second + width], h)
+        assert torch.equal(a[:, first:first + width], x) and torch.equal(b[:, first:first + width], y)
+        assert (a[:, width:width + 8] == 9).all() and (b[:, 2 * width + 8:] == 9).all() and (a[:, 2 * width + 8:] == 9).all()
